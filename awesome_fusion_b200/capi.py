@@ -21,6 +21,7 @@ FLAG_DUMP_DECODE_PAIRING = 16
 FLAG_GROUP_EXACT = 32
 FLAG_PDL = 64
 ACT_NONE, ACT_SILU = 0, 1
+MOE_MAX_EXPERTS, MOE_MAX_TOP_K = 1024, 32
 IPC_HANDLE_BYTES = 64
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -31,7 +32,8 @@ EXPORTS = [
     "afb_free_host", "afb_memcpy_h2d", "afb_memcpy_d2h", "afb_memcpy_d2d", "afb_memset", "afb_event_create",
     "afb_event_record", "afb_event_sync", "afb_event_elapsed_ms", "afb_event_destroy", "afb_stream_create",
     "afb_stream_sync", "afb_stream_destroy", "afb_device_sync", "afb_gemm_launch", "afb_gemm_resolve_variant",
-    "afb_gemm_host", "afb_gemm_host_async", "afb_gemm_host_wait", "afb_gemm_launch_static", "afb_prepack", "afb_prepack_gated", "afb_gemm_fused_launch", "afb_dequant_dump", "afb_read_status", "afb_ipc_export", "afb_ipc_import", "afb_ipc_release",
+    "afb_gemm_host", "afb_gemm_host_async", "afb_gemm_host_wait", "afb_gemm_launch_static", "afb_prepack", "afb_prepack_gated", "afb_gemm_fused_launch",
+    "afb_moe_route_workspace", "afb_moe_route_launch", "afb_expert_gemm_launch", "afb_moe_combine_launch", "afb_moe_abi_sizes", "afb_dequant_dump", "afb_read_status", "afb_ipc_export", "afb_ipc_import", "afb_ipc_release",
     "afb_ksplit_allreduce_launch", "afb_cast_f32_to_bf16", "afb_ksplit_tile_info", "afb_gemm_launch_tiles", "afb_ksplit_tile_allreduce_launch", "afb_gemm_launch_push", "afb_abi_sizes",
     "afb_dist_init", "afb_dist_world", "afb_dist_stream", "afb_dist_gemm_launch", "afb_dist_sync", "afb_dist_finalize", "afb_dist_split_range",
     "afb_ksplit_sub_info", "afb_gemm_launch_push_pipelined", "afb_ksplit_sub_allreduce_launch", "afb_gemm_launch_push_exchange", "afb_probe_launch", "afb_phase_timestamps", "afb_status_string", "afb_last_cuda_error", "afb_last_cuda_error_string", "afb_launch_count", "afb_stream_launch_count", "afb_pair_launch_count", "afb_version",
@@ -61,6 +63,29 @@ class FusedArgs(ctypes.Structure):
     """``afb_fused_args``: a GEMM plus its fused epilogue (bias, activation, gate * up, residual)."""
     _fields_ = [("gemm", GemmArgs), ("gated", ctypes.c_uint32), ("activation", ctypes.c_uint32), ("ptr_bias", ctypes.c_void_p),
                 ("ptr_residual", ctypes.c_void_p), ("ld_residual", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
+
+
+class MoeRouteArgs(ctypes.Structure):
+    """``afb_moe_route_args``: logits -> picks, weights and the pairs sorted by expert."""
+    _fields_ = [("ptr_logits", ctypes.c_void_p), ("ptr_ids", ctypes.c_void_p), ("ptr_weights", ctypes.c_void_p), ("ptr_offsets", ctypes.c_void_p),
+                ("ptr_row_pair", ctypes.c_void_p), ("ptr_pair_row", ctypes.c_void_p), ("ptr_workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_uint64), ("tokens", ctypes.c_uint32), ("experts", ctypes.c_uint32), ("ld_logits", ctypes.c_uint32),
+                ("top_k", ctypes.c_uint32), ("logits_f32", ctypes.c_uint32), ("renormalize", ctypes.c_uint32), ("reserved", ctypes.c_uint64)]
+
+
+class ExpertGemmArgs(ctypes.Structure):
+    """``afb_expert_gemm_args``: the products grouped by expert."""
+    _fields_ = [("gemm", GemmArgs), ("ptr_offsets", ctypes.c_void_p), ("ptr_row_pair", ctypes.c_void_p), ("experts", ctypes.c_uint32),
+                ("top_k", ctypes.c_uint32), ("a_rows", ctypes.c_uint32), ("gated", ctypes.c_uint32), ("activation", ctypes.c_uint32),
+                ("reserved", ctypes.c_uint32)]
+
+
+class MoeCombineArgs(ctypes.Structure):
+    """``afb_moe_combine_args``: the weighted sum of the picked experts' answers."""
+    _fields_ = [("ptr_out", ctypes.c_void_p), ("ptr_y", ctypes.c_void_p), ("ptr_weights", ctypes.c_void_p), ("ptr_pair_row", ctypes.c_void_p),
+                ("ptr_residual", ctypes.c_void_p), ("tokens", ctypes.c_uint32), ("top_k", ctypes.c_uint32), ("rows", ctypes.c_uint32),
+                ("n", ctypes.c_uint32), ("ld_out", ctypes.c_uint32), ("ld_y", ctypes.c_uint32), ("ld_residual", ctypes.c_uint32),
+                ("reserved", ctypes.c_uint32)]
 
 
 def library_path() -> str:
@@ -118,6 +143,11 @@ class Library:
         L.afb_prepack.argtypes = [ctypes.POINTER(GemmArgs), vp, ctypes.c_uint32, vp]
         L.afb_prepack_gated.argtypes = [ctypes.POINTER(GemmArgs), vp, vp, vp, vp, ctypes.c_uint32, vp, vp, vp]
         L.afb_gemm_fused_launch.argtypes = [ctypes.POINTER(FusedArgs), vp]
+        L.afb_moe_route_workspace.argtypes = [ctypes.c_uint32, ctypes.c_uint32, ctypes.POINTER(ctypes.c_uint64)]
+        L.afb_moe_route_launch.argtypes = [ctypes.POINTER(MoeRouteArgs), vp]
+        L.afb_expert_gemm_launch.argtypes = [ctypes.POINTER(ExpertGemmArgs), vp]
+        L.afb_moe_combine_launch.argtypes = [ctypes.POINTER(MoeCombineArgs), vp]
+        L.afb_moe_abi_sizes.argtypes = [ctypes.POINTER(ctypes.c_uint32)]
         L.afb_read_status.argtypes = [ctypes.POINTER(ctypes.c_int32)]
         L.afb_ipc_export.argtypes = [vp, ctypes.c_char_p]
         L.afb_ipc_import.argtypes = [ctypes.c_char_p, ctypes.POINTER(vp)]
@@ -290,6 +320,47 @@ class Library:
 
     def gemm_fused_launch(self, fused_args, stream=None):
         self.check(self.lib.afb_gemm_fused_launch(ctypes.byref(fused_args), stream), "afb_gemm_fused_launch")
+
+    # ---- a mixture-of-experts layer ----------------------------------------------
+    def moe_route_workspace(self, tokens, experts):
+        """Bytes of device memory that a route of this size needs."""
+        n = ctypes.c_uint64(0)
+        self.check(self.lib.afb_moe_route_workspace(tokens, experts, ctypes.byref(n)), "afb_moe_route_workspace")
+        return n.value
+
+    @staticmethod
+    def make_moe_route_args(logits, ids, weights, offsets, row_pair, pair_row, *, tokens, experts, top_k, ld_logits=None, logits_f32=False,
+                            renormalize=True, workspace=None, workspace_bytes=0):
+        return MoeRouteArgs(_ptr(logits), _ptr(ids), _ptr(weights), _ptr(offsets), _ptr(row_pair), _ptr(pair_row), _ptr(workspace), workspace_bytes,
+                            tokens, experts, experts if ld_logits is None else ld_logits, top_k, int(logits_f32), int(renormalize), 0)
+
+    def moe_route_launch_status(self, args, stream=None):
+        return self.lib.afb_moe_route_launch(ctypes.byref(args), stream)
+
+    def moe_route_launch(self, args, stream=None):
+        self.check(self.lib.afb_moe_route_launch(ctypes.byref(args), stream), "afb_moe_route_launch")
+
+    @staticmethod
+    def make_expert_gemm_args(gemm_args, offsets, *, experts, row_pair=None, top_k=1, a_rows=None, gated=False, activation=ACT_NONE):
+        """gemm_args: make_args with m rows of C and n rows of B per expert.  a_rows: rows of A (default: m)."""
+        return ExpertGemmArgs(gemm_args, _ptr(offsets), _ptr(row_pair), experts, top_k, gemm_args.m if a_rows is None else a_rows, int(gated), activation, 0)
+
+    def expert_gemm_launch_status(self, args, stream=None):
+        return self.lib.afb_expert_gemm_launch(ctypes.byref(args), stream)
+
+    def expert_gemm_launch(self, args, stream=None):
+        self.check(self.lib.afb_expert_gemm_launch(ctypes.byref(args), stream), "afb_expert_gemm_launch")
+
+    @staticmethod
+    def make_moe_combine_args(out, y, weights, pair_row, *, tokens, top_k, rows, n, ld_out=None, ld_y=None, residual=None, ld_residual=None):
+        return MoeCombineArgs(_ptr(out), _ptr(y), _ptr(weights), _ptr(pair_row), _ptr(residual), tokens, top_k, rows, n, n if ld_out is None else ld_out,
+                              n if ld_y is None else ld_y, n if ld_residual is None else ld_residual, 0)
+
+    def moe_combine_launch_status(self, args, stream=None):
+        return self.lib.afb_moe_combine_launch(ctypes.byref(args), stream)
+
+    def moe_combine_launch(self, args, stream=None):
+        self.check(self.lib.afb_moe_combine_launch(ctypes.byref(args), stream), "afb_moe_combine_launch")
 
     def dequant_dump(self, args, out, stream=None):
         self.check(self.lib.afb_dequant_dump(ctypes.byref(args), _ptr(out), stream), "afb_dequant_dump")

@@ -17,7 +17,8 @@ the call is stream-ordered with the surrounding torch work and can be captured i
 """
 import torch
 
-from .capi import ENC_OFFSET, ENC_TWOS, FLAG_PDL, SCALE_BF16, SCALE_F32, AfbError, load
+from .capi import (ACT_NONE, ACT_SILU, ENC_OFFSET, ENC_TWOS, FLAG_PDL, LAYOUT_COL, LAYOUT_COL_PACKED, MOE_MAX_EXPERTS, MOE_MAX_TOP_K, SCALE_BF16,
+                   SCALE_F32, AfbError, load)
 
 _LIB_NAME = "afb::bf16_aintb_gemm"
 
@@ -98,3 +99,154 @@ class DecodeGraph:
     def replay(self):
         self.graph.replay()
         return self.out
+
+
+# ---- a mixture-of-experts layer --------------------------------------------------------------------------------------------------------
+#
+#     weights, ids, offsets, row_pair, pair_row = torch.ops.afb.moe_route(logits, top_k, renormalize)
+#     h = torch.ops.afb.expert_gemm(x, w1, s1, None, offsets, row_pair, top_k, bits, group_size, offset_binary, packed, True)   # silu(gate) * up
+#     y = torch.ops.afb.expert_gemm(h, w2, s2, None, offsets, None, 1, bits, group_size, offset_binary, packed, False)
+#     out = torch.ops.afb.moe_combine(y, weights, pair_row, residual)
+#
+# include/afb_capi.h says what each computes.  Weights are [experts, N, K * bits / 8], scales [experts, N] or [experts, N, K / group_size],
+# zero-points (optional) uint8 of the scales' shape.  No host synchronisation; zero tokens are taken.
+
+def _on(t, name, device, dtypes, dim=None):
+    if t.device != device or t.dtype not in dtypes or (dim is not None and t.dim() != dim):
+        raise ValueError(f"{name} must be a {'/'.join(str(d).split('.')[-1] for d in dtypes)} tensor{'' if dim is None else f' of {dim} dimensions'} on {device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _run(device, call):
+    """call(library, stream) on the tensors' device."""
+    dev = device.index if device.index is not None else torch.cuda.current_device()
+    lib = load()
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            lib.init(dev)
+            return call(lib, torch.cuda.current_stream(dev).cuda_stream)
+    lib.init(dev)
+    return call(lib, torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _route_shapes(logits, top_k):
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or logits.shape[1] == 0:
+        raise ValueError("logits must be an fp32 or bf16 [tokens, experts] tensor")
+    tokens, experts = logits.shape
+    if not 1 <= top_k <= min(experts, MOE_MAX_TOP_K) or experts > MOE_MAX_EXPERTS:
+        raise ValueError(f"1 <= top_k <= min(experts, {MOE_MAX_TOP_K}) and experts <= {MOE_MAX_EXPERTS}")
+    i32 = torch.int32
+    return (logits.new_empty((tokens, top_k), dtype=torch.float32), logits.new_empty((tokens, top_k), dtype=i32), logits.new_empty((experts + 1,), dtype=i32),
+            logits.new_empty((tokens * top_k,), dtype=i32), logits.new_empty((tokens, top_k), dtype=i32))
+
+
+@torch.library.custom_op("afb::moe_route", mutates_args=(), device_types="cuda")
+def moe_route(logits: torch.Tensor, top_k: int, renormalize: bool = True) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    weights, ids, offsets, row_pair, pair_row = out = _route_shapes(logits, top_k)
+    tokens, experts = logits.shape
+    if logits.stride(1) != 1 or (tokens > 1 and logits.stride(0) < experts):
+        raise ValueError("logits: rows of consecutive experts that do not overlap")
+
+    def call(lib, stream):
+        room = lib.moe_route_workspace(tokens, experts)
+        work = logits.new_empty((room,), dtype=torch.uint8) if room else None
+        lib.moe_route_launch(lib.make_moe_route_args(logits, ids, weights, offsets, row_pair, pair_row, tokens=tokens, experts=experts, top_k=top_k,
+                                                     ld_logits=logits.stride(0) if tokens > 1 else experts, logits_f32=logits.dtype == torch.float32,
+                                                     renormalize=renormalize, workspace=work, workspace_bytes=room), stream)
+    _run(logits.device, call)
+    return out
+
+
+@moe_route.register_fake
+def _(logits, top_k, renormalize=True):
+    return _route_shapes(logits, top_k)
+
+
+def _expert_shapes(a, b, scale, zero, offsets, row_pair, top_k, bits, group_size, gated):
+    if bits not in (4, 8):
+        raise ValueError("bits must be 4 or 8")
+    if a.dtype != torch.bfloat16 or a.dim() != 2:
+        raise ValueError("a must be a bf16 [rows, K] tensor")
+    k = a.shape[1]
+    if b.dim() != 3 or b.dtype not in (torch.int8, torch.uint8) or b.shape[2] * (8 // bits) != k:
+        raise ValueError("b must be an int8 / uint8 [experts, N, K * bits / 8] tensor")
+    experts, n = b.shape[:2]
+    if gated and n % 2:
+        raise ValueError("gated: N counts gate and up rows in turn")
+    want = (experts, n) if group_size == 0 else (experts, n, k // group_size) if group_size > 0 and k % group_size == 0 else None
+    for name, t, dtypes in (("scale", scale, (torch.float32, torch.bfloat16)), ("zero", zero, (torch.uint8, torch.int8))):
+        if t is not None and (tuple(t.shape) != want or t.dtype not in dtypes):
+            raise ValueError(f"{name} must be [experts, N] (group_size = 0) or [experts, N, K / group_size]")
+    if offsets.dtype != torch.int32 or offsets.shape != (experts + 1,):
+        raise ValueError("offsets must be int32 [experts + 1]")
+    if row_pair is not None and (row_pair.dtype != torch.int32 or row_pair.dim() != 1):
+        raise ValueError("row_pair must be int32 [rows]")
+    if top_k < 1 or (row_pair is None and top_k != 1):
+        raise ValueError("top_k divides row_pair; without one it is 1")
+    return a.new_empty((a.shape[0] if row_pair is None else row_pair.shape[0], n // 2 if gated else n))
+
+
+@torch.library.custom_op("afb::expert_gemm", mutates_args=(), device_types="cuda")
+def expert_gemm(a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None, offsets: torch.Tensor, row_pair: torch.Tensor | None,
+                top_k: int, bits: int, group_size: int, offset_binary: bool, packed: bool = False, gated: bool = False) -> torch.Tensor:
+    """The products grouped by expert; gated: silu(gate) * up of interleaved rows.  Rows behind offsets[experts] are not written."""
+    out = _expert_shapes(a, b, scale, zero, offsets, row_pair, top_k, bits, group_size, gated)
+    for name, t in (("a", a), ("b", b), ("scale", scale), ("zero", zero), ("offsets", offsets), ("row_pair", row_pair)):
+        if t is not None:
+            _on(t, name, a.device, (t.dtype,))
+    experts, n = b.shape[:2]
+
+    def call(lib, stream):
+        gemm = lib.make_args(out, a, b, scale, out.shape[0], n, a.shape[1], ldc=out.shape[1], bits=bits, group=group_size, zero=zero,
+                             layout=LAYOUT_COL_PACKED if packed else LAYOUT_COL, encoding=ENC_OFFSET if offset_binary else ENC_TWOS,
+                             scale_dtype=SCALE_BF16 if scale.dtype == torch.bfloat16 else SCALE_F32)
+        lib.expert_gemm_launch(lib.make_expert_gemm_args(gemm, offsets, experts=experts, row_pair=row_pair, top_k=top_k, a_rows=a.shape[0], gated=gated,
+                                                         activation=ACT_SILU if gated else ACT_NONE), stream)
+    _run(a.device, call)
+    return out
+
+
+@expert_gemm.register_fake
+def _(a, b, scale, zero, offsets, row_pair, top_k, bits, group_size, offset_binary, packed=False, gated=False):
+    return _expert_shapes(a, b, scale, zero, offsets, row_pair, top_k, bits, group_size, gated)
+
+
+def _combine_shapes(y, weights, pair_row, residual):
+    if y.dtype != torch.bfloat16 or y.dim() != 2 or y.shape[1] == 0:
+        raise ValueError("y must be a bf16 [rows, N] tensor")
+    if weights.dtype != torch.float32 or pair_row.dtype != torch.int32 or weights.dim() != 2 or weights.shape != pair_row.shape or weights.shape[1] == 0:
+        raise ValueError("weights (fp32) and pair_row (int32) must be [tokens, top_k]")
+    out = y.new_empty((weights.shape[0], y.shape[1]))
+    if residual is not None and (residual.dtype != torch.bfloat16 or residual.shape != out.shape):
+        raise ValueError("residual must be bf16 [tokens, N]")
+    return out
+
+
+@torch.library.custom_op("afb::moe_combine", mutates_args=(), device_types="cuda")
+def moe_combine(y: torch.Tensor, weights: torch.Tensor, pair_row: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """sum over the picks of weight * the expert's answer, plus the residual."""
+    out = _combine_shapes(y, weights, pair_row, residual)
+    for name, t in (("y", y), ("weights", weights), ("pair_row", pair_row), ("residual", residual)):
+        if t is not None:
+            _on(t, name, y.device, (t.dtype,))
+
+    def call(lib, stream):
+        lib.moe_combine_launch(lib.make_moe_combine_args(out, y, weights, pair_row, tokens=out.shape[0], top_k=weights.shape[1], rows=y.shape[0],
+                                                         n=y.shape[1], residual=residual), stream)
+    _run(y.device, call)
+    return out
+
+
+@moe_combine.register_fake
+def _(y, weights, pair_row, residual=None):
+    return _combine_shapes(y, weights, pair_row, residual)
+
+
+def moe_mlp(x, logits, w1, s1, w2, s2, top_k, bits=8, group_size=0, offset_binary=False, packed=False, renormalize=True, zero1=None, zero2=None, residual=None):
+    """A gated mixture-of-experts MLP on quantised weights: x bf16 [tokens, K], router logits [tokens, experts], w1 [experts, 2 F, K] with gate and
+    up rows in turn (afb_prepack_gated lays them out), w2 [experts, K, F].  bf16 [tokens, K], plus the residual."""
+    weights, _, offsets, row_pair, pair_row = torch.ops.afb.moe_route(logits, top_k, renormalize)
+    h = torch.ops.afb.expert_gemm(x, w1, s1, zero1, offsets, row_pair, top_k, bits, group_size, offset_binary, packed, True)
+    y = torch.ops.afb.expert_gemm(h, w2, s2, zero2, offsets, None, 1, bits, group_size, offset_binary, packed, False)
+    return torch.ops.afb.moe_combine(y, weights, pair_row, residual)

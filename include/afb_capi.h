@@ -203,6 +203,85 @@ int afb_gemm_fused_launch(const afb_fused_args* args, void* stream);
  * (and out_zero).  gate->n is N, the output has 2N rows.  Asynchronous on `stream`. */
 int afb_prepack_gated(const afb_gemm_args* gate, const void* b_up, const void* scale_up, const void* zero_up, void* out_b,
                       uint32_t out_ldb, void* out_scale, void* out_zero, void* stream);
+/* ---- a mixture-of-experts layer on quantised weights ------------------------------- */
+/* The reference's purpose is "gemm fusion for llm" (README.md:2); its GEMM serves dense layers.  These entry points serve the layer in which
+ * every token picks a few of `experts` weight matrices:
+ *     afb_moe_route_launch    logits -> picks, weights, and the pairs (token, pick) sorted by expert
+ *     afb_expert_gemm_launch  the products grouped by expert, once for gate and up projection (gated), once for the down projection
+ *     afb_moe_combine_launch  the weighted sum of the picked experts' answers
+ * All four launches of a layer go to one stream; nothing is copied to the host, no size depends on the picks, nothing is allocated, so
+ * the layer can be captured in a graph.  A pair is numbered token * top_k + pick; the ROW of a pair is its place in the sorted order.
+ *
+ * afb_moe_route_launch.  For every token the top_k largest logits in falling order, of equal ones the lower expert first (-0 equals 0).
+ * A logit that is -inf or NaN is masked: its expert is never picked.  Where fewer than top_k experts are left (none in a token of padding)
+ * the remaining ids are -1, with weight 0, and their pairs have no row.
+ *     weight = exp(logit - max) / sum of exp(l - max), over the picked experts (renormalize = 1) or over all (0);  in fp32; a logit of +inf
+ *     counts as equal to the largest (exp(0)).
+ * The pairs are sorted by expert, those of one expert by their number: the result is the same in every run. */
+#define AFB_MOE_MAX_EXPERTS 1024u
+#define AFB_MOE_MAX_TOP_K   32u
+typedef struct afb_moe_route_args {
+    const void* ptr_logits;    /* [tokens, experts], pitch ld_logits elements; bf16 or fp32                       */
+    int32_t*  ptr_ids;         /* [tokens, top_k]    picked experts, -1: none left                                 */
+    float*    ptr_weights;     /* [tokens, top_k]                                                                  */
+    int32_t*  ptr_offsets;     /* [experts + 1]      rows offsets[e] .. offsets[e + 1] are expert e's              */
+    int32_t*  ptr_row_pair;    /* [tokens * top_k]   pair of every row, -1 behind the last row                      */
+    int32_t*  ptr_pair_row;    /* [tokens, top_k]    row of every pair, -1 where it has none                        */
+    void*     ptr_workspace;   /* afb_moe_route_workspace() bytes, 4-byte aligned, used during the launch only       */
+    uint64_t  workspace_bytes;
+    uint32_t  tokens;          /* 0: only the offsets are written; tokens * top_k < 2^31                            */
+    uint32_t  experts;         /* 1 .. AFB_MOE_MAX_EXPERTS                                                          */
+    uint32_t  ld_logits;       /* elements, >= experts                                                              */
+    uint32_t  top_k;           /* 1 .. AFB_MOE_MAX_TOP_K, <= experts                                                */
+    uint32_t  logits_f32;      /* 1: fp32, 0: bf16                                                                  */
+    uint32_t  renormalize;     /* 0 / 1                                                                             */
+    uint64_t  reserved;        /* must be 0                                                                         */
+} afb_moe_route_args;
+/* Bytes of device memory that a route of this size needs at ptr_workspace (0: none; then NULL will do).  Needs no GPU. */
+int afb_moe_route_workspace(uint32_t tokens, uint32_t experts, uint64_t* bytes);
+int afb_moe_route_launch(const afb_moe_route_args* args, void* stream);
+/* afb_expert_gemm_launch.  gemm describes one expert's product, with
+ *     m        rows of C: the pairs, an upper bound of offsets[experts]; rows from offsets[experts] on are left as they are
+ *     n, ldb   rows of B per expert; expert e's B begins e * n rows behind ptr_b, its scales (and zero-points) likewise: [experts, n] or
+ *              [experts, n, k / group_size]
+ *     b_layout AFB_LAYOUT_COL or AFB_LAYOUT_COL_PACKED (afb_prepack / afb_prepack_gated of all experts at once: a matrix of experts * n rows)
+ *     group_size 0, or a power of two of at least 64;  k a multiple of 64 (int8) or 128 (int4);  lda a multiple of 8, A 16-byte aligned, rows
+ *              of B and ptr_b 16-byte aligned; any n and ldc.  Otherwise AFB_ERR_UNSUPPORTED
+ *     variant  AFB_VARIANT_AUTO, AFB_VARIANT_DECODE (form for few rows per expert: weights streamed through registers) or
+ *              AFB_VARIANT_PREFILL (form for many: tcgen05);  flags 0.
+ *     C[r,:] = f(A[row(r),:] x dequant(B[e])^T)   for offsets[e] <= r < offsets[e + 1]
+ *     row(r) = ptr_row_pair[r] / top_k (the first product: A holds the tokens), or r where ptr_row_pair is NULL (the second one)
+ *     f: nothing, the activation, or gated: act(v[2i]) * v[2i + 1] into n / 2 columns
+ * in fp32 from the fp32 sums; group scales multiply the fp32 sum of each group in both forms; rounded to bf16 once.
+ * The offsets are read on the GPU.  They must not fall; values outside 0 .. m are taken as the nearer end.  A row(r) outside
+ * 0 .. a_rows - 1 reads as a row of zeros. */
+typedef struct afb_expert_gemm_args {
+    afb_gemm_args  gemm;
+    const int32_t* ptr_offsets;    /* [experts + 1] */
+    const int32_t* ptr_row_pair;   /* [m], or NULL  */
+    uint32_t experts;              /* 1 .. AFB_MOE_MAX_EXPERTS */
+    uint32_t top_k;                /* divisor of ptr_row_pair; 1 where it is NULL */
+    uint32_t a_rows;               /* rows of A */
+    uint32_t gated;                /* 0 / 1 */
+    uint32_t activation;           /* AFB_ACT_* */
+    uint32_t reserved;             /* must be 0 */
+} afb_expert_gemm_args;
+int afb_expert_gemm_launch(const afb_expert_gemm_args* args, void* stream);
+/* afb_moe_combine_launch.  out[t,:] = sum over j of weights[t,j] * Y[pair_row[t,j],:] + residual[t,:], in fp32, j in order, rounded to bf16
+ * once.  A pair_row outside 0 .. rows - 1 adds nothing, whatever its weight.  out may be the residual, not Y. */
+typedef struct afb_moe_combine_args {
+    void*          ptr_out;        /* bf16 [tokens, n], ld_out */
+    const void*    ptr_y;          /* bf16 [rows, n], ld_y */
+    const float*   ptr_weights;    /* [tokens, top_k] */
+    const int32_t* ptr_pair_row;   /* [tokens, top_k] */
+    const void*    ptr_residual;   /* bf16 [tokens, n], ld_residual; or NULL */
+    uint32_t tokens, top_k, rows, n;
+    uint32_t ld_out, ld_y, ld_residual;
+    uint32_t reserved;             /* must be 0 */
+} afb_moe_combine_args;
+int afb_moe_combine_launch(const afb_moe_combine_args* args, void* stream);
+/* sizeof(afb_moe_route_args), sizeof(afb_expert_gemm_args), sizeof(afb_moe_combine_args) as compiled, see afb_abi_sizes. */
+int afb_moe_abi_sizes(uint32_t sizes[3]);
 /* Dequantised weights exactly as the kernels feed them to the tensor cores:
  * out is bf16 with B's logical shape and layout ([N,K] ld=K for COL, [K,N] ld=N for ROW).
  * group_size == 0: the exact integer value; else bf16_rn(float(q) * float(scale)).
