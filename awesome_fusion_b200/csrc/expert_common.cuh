@@ -1,6 +1,7 @@
 // Shared by the two forms of the products grouped by expert (expert_few.cu, expert_many.cu): the parameter block and the way a CTA finds its
 // tile.  How many rows an expert has is known on the GPU only; the launch covers the most tiles there can be, the rest find nothing to do.
 #pragma once
+#include "activation.cuh"
 #include "afb_internal.h"
 
 namespace afb {
@@ -74,8 +75,10 @@ __device__ __forceinline__ uint32_t source_row(const ExpertParams& p, uint32_t r
     return pair < 0 ? 0xffffffffu : (uint32_t)pair / p.top_k;
 }
 
-__device__ __forceinline__ float silu(float v) { return v / (1.f + __expf(-v)); }
+__device__ __forceinline__ float silu(float v) { return v * sigmoid(v); }
 
+// `bits`, `group`: of the weights.  The form for many rows takes no empty A (a tensor map has at least one row).
+int launch_expert_many(const ExpertParams& p, uint32_t bits, uint32_t group, DeviceCtx* ctx, cudaStream_t s);
 int launch_expert_few(const ExpertParams& p, uint32_t bits, uint32_t group, DeviceCtx* ctx, cudaStream_t s);
 
 }  // namespace afb

@@ -1,0 +1,553 @@
+// Products grouped by expert, many rows per expert (afb_expert_gemm_launch): two SMs on one tile, as in the pair form of the dense product
+// (pair.cu; reference counterpart of the product: bf16gemm_kernel_gfx90a.s:184-636, which has no experts).
+//
+// D[n, r] = sum_k W[e][n,k] * A[row(r),k] with the unpacked weights as the tensor-memory operand.  A cluster of two CTAs owns 256 channels of
+// one expert x one strip of its rows: each unpacks its own 128 channels into its own tensor memory, each gathers half of the strip's rows of A, and
+// one tcgen05.mma.cta_group::2 reads both halves.  An expert's rows are cut into strips of equal height, a multiple of 32.
+//
+//   warp 0        TMA: raw weight blocks, 128 channels x 128 bytes, 128-byte swizzle
+//   warp 1        TMA gather of this CTA's half of the strip: four rows of 64 k per instruction and lane, 128-byte swizzle
+//   warps 2, 3    rank 0: tcgen05.mma 256 x height x 16;  rank 1, warp 2: reports to rank 0 that its half of a step is complete
+//   warps 4-11    epilogue, two per lane quarter: accumulator -> registers -> (accumulator free) -> shared memory -> C
+//   warps 12-27   converters: four groups of four warps; group g takes every fourth step of k (KS = 128 or 64 wide)
+//
+// Scales per channel: the sum over all of K stays in the accumulator, strips of up to 256 rows.
+// Scales per group: a weight times its scale has no room in a bf16 (up to 8 x 8 significant bits), and rounding it there costs as much
+// accuracy as the rounding of the result.  So every step has an accumulator of its own, two take turns, and the epilogue warps add scale * sum in
+// fp32 registers: strips of up to 128 rows (64 sums a thread).  A step is then 512 cycles of tensor work, less than one warp needs to issue it
+// (wait 80, eight MMAs 480, two commits 360): two warps issue, one per accumulator.
+//
+// A table in shared memory says where each expert's rows and strips begin; every role walks the same tiles from it: tile t = worker, worker +
+// workers, ...; inside an expert the channels advance, strip fastest, so that its weights are read from HBM once.
+#include "dequant.cuh"
+#include "expert_common.cuh"
+#include "stream_common.cuh"
+
+namespace afb {
+namespace {
+
+constexpr int kFirstEpi = 4, kEpiWarps = 8, kFirstConv = kFirstEpi + kEpiWarps;
+constexpr int kManyThreads = 32 * (kFirstConv + 4 * kGroups);   // 896: launched with 72 registers a thread
+constexpr uint32_t kRegsCtrl = 56, kRegsEpi = 112, kRegsConv = 56;
+static_assert(128 * kRegsCtrl + 32 * kEpiWarps * kRegsEpi + 128 * kGroups * kRegsConv <= 72 * kManyThreads, "shares of the registers");
+constexpr int kMaxRaw = 12, kMaxSlots = 8, kMaxAcc = 2;
+__host__ __device__ constexpr uint32_t slots(int ks) { return ks == 128 ? 4 : 6; }   // steps under way, in 256 columns at most
+constexpr uint32_t kTmemCols = 512;
+constexpr int kBars = 2 * (kMaxRaw + kMaxSlots + kMaxAcc);
+constexpr int kOffMisc = kBars * 8, kOffOut = 1024;
+constexpr int kOutBytes = 16 * 32 * 2;   // one block of the result: 16 rows x 32 channels; two per epilogue warp
+constexpr int kOffTable = kOffOut + kEpiWarps * 2 * kOutBytes;
+static_assert(kOffMisc + 16 <= kOffOut, "shared memory layout");
+constexpr uint32_t kUnit = 32;           // rows: 16 per epilogue warp
+
+struct ManyParams {
+    ExpertParams x;
+    uint32_t steps;           // along K
+    uint32_t raw_stages, accs;
+    uint32_t slot_first;      // converters wait for their slot before they wait for their raw block
+    uint32_t off_raw;         // behind the table
+    uint32_t c_vec;           // 16-byte stores of C
+    int32_t* status;
+};
+
+struct Strip { uint32_t expert, row0, rows, height, n0; };   // n0: of this CTA's 128 channels
+
+template <int BITS, bool GROUPED, int KS>
+__global__ void __launch_bounds__(kManyThreads, 1)
+expert_many_kernel(const __grid_constant__ CUtensorMap tmap_act, const __grid_constant__ CUtensorMap tmap_w, const ManyParams p) {
+    constexpr uint32_t SPB = (BITS == 8 ? 128 : 256) / KS;   // steps per raw block
+    constexpr uint32_t kSlotCols = KS / 2;                   // TMEM columns of a step's weights
+    constexpr uint32_t kSlots = slots(KS);
+    constexpr uint32_t kIssuers = GROUPED ? 2 : 1;
+    extern __shared__ uint8_t smem_raw_base[];
+    const uint32_t smem_base = (ptx::smem_u32(smem_raw_base) + 1023u) & ~1023u;
+    uint8_t* smem_gen = smem_raw_base + (smem_base - ptx::smem_u32(smem_raw_base));
+    auto bar = [&](uint32_t i) { return smem_base + 8u * i; };
+    auto raw_full = [&](uint32_t s) { return bar(s); };
+    auto raw_empty = [&](uint32_t s) { return bar(kMaxRaw + s); };
+    auto step_full = [&](uint32_t s) { return bar(2 * kMaxRaw + s); };                // weights in TMEM, activations in shared memory; rank 0: of both CTAs
+    auto step_empty = [&](uint32_t s) { return bar(2 * kMaxRaw + kMaxSlots + s); };   // the MMAs of the step are done with both
+    auto acc_full = [&](uint32_t s) { return bar(2 * (kMaxRaw + kMaxSlots) + s); };
+    auto acc_empty = [&](uint32_t s) { return bar(2 * (kMaxRaw + kMaxSlots) + kMaxAcc + s); };   // rank 0: of both CTAs
+    volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(smem_gen + kOffMisc);   // TMEM base, abort flag
+    volatile uint32_t* abort_flag = misc + 1;
+    uint32_t* strips_before = reinterpret_cast<uint32_t*>(smem_gen + kOffTable);   // [experts + 1]
+    uint32_t* first_row = strips_before + p.x.experts + 1;                         // [experts]
+    uint32_t* row_count = first_row + p.x.experts;                                 // [experts]
+    const uint32_t act_stride = p.x.tile_rows * KS;   // bytes of one CTA's half of a step, at most
+    const uint32_t off_act = p.off_raw + p.raw_stages * kRawBytes;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = ptx::cluster_rank(), worker = blockIdx.x >> 1, workers = gridDim.x >> 1;
+
+    if (warp == 0 && lane == 0) {
+        for (uint32_t s = 0; s < p.raw_stages; ++s) { ptx::mbar_init(raw_full(s), 1); ptx::mbar_init(raw_empty(s), 4 * SPB); }
+        for (uint32_t s = 0; s < kSlots; ++s) { ptx::mbar_init(step_full(s), 4 + 1 + (rank == 0 ? 1 : 0)); ptx::mbar_init(step_empty(s), 1); }
+        for (uint32_t s = 0; s < p.accs; ++s) { ptx::mbar_init(acc_full(s), 1); ptx::mbar_init(acc_empty(s), 2 * kEpiWarps); }
+        *abort_flag = 0;
+        ptx::fence_mbar_init();
+        ptx::prefetch_tmap(&tmap_act);
+        ptx::prefetch_tmap(&tmap_w);
+    }
+    if (warp == 2) {
+        ptx::tmem_alloc_pair(ptx::smem_u32(const_cast<uint32_t*>(misc)), kTmemCols);
+        ptx::tmem_relinquish_pair();
+    }
+    if (warp == 3) {   // the table: 32 experts at a time
+        uint32_t before = 0;
+        for (uint32_t e0 = 0; e0 < p.x.experts; e0 += 32) {
+            const uint32_t e = e0 + lane;
+            uint32_t lo = 0, hi = 0;
+            if (e < p.x.experts) {
+                lo = clamp_offset(__ldg(p.x.offsets + e), p.x.m);
+                hi = max(lo, clamp_offset(__ldg(p.x.offsets + e + 1), p.x.m));
+            }
+            const uint32_t mine = (hi - lo + p.x.tile_rows - 1) / p.x.tile_rows;
+            uint32_t upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
+            }
+            if (e < p.x.experts) { strips_before[e] = before + upto - mine; first_row[e] = lo; row_count[e] = hi - lo; }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (lane == 0) strips_before[p.x.experts] = before;
+    }
+    __syncwarp();
+    ptx::tc_fence_before_sync();
+    __syncthreads();       // the table
+    ptx::cluster_arrive();
+    ptx::cluster_wait();   // both CTAs' barriers are there
+    ptx::tc_fence_after_sync();
+    constexpr uint32_t tmem_base = 0;   // all 512 columns are this CTA's: the allocation starts at column 0
+    const uint32_t slot_base = tmem_base + kTmemCols - kSlots * kSlotCols;   // accumulators from column 0, slots at the end
+    const uint32_t acc_cols = p.x.tile_rows;
+
+    auto give_up = [&](int where, uint32_t a, uint32_t b) {
+        if (!*abort_flag) { report_timeout(p.status, where, (int)a, (int)b); *abort_flag = 1; }
+    };
+    const uint32_t tiles = strips_before[p.x.experts] * p.x.n_blocks;   // < 2^31, the launcher sees to it
+    uint32_t t = worker;   // every role of both CTAs walks the same list of tiles
+    auto next = [&](Strip& s) {
+        if (t >= tiles) return false;
+        const uint32_t q = t / p.x.n_blocks;
+        uint32_t lo = 0, hi = p.x.experts;   // the expert with strips_before[e] <= q < strips_before[e + 1]
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (strips_before[mid] <= q) lo = mid; else hi = mid;
+        }
+        const uint32_t first = strips_before[lo], of = strips_before[lo + 1] - first, r = t - first * p.x.n_blocks, nt = r / of, i = r - nt * of;
+        const uint32_t all = row_count[lo], height = ((all + of - 1) / of + kUnit - 1) / kUnit * kUnit;
+        s.expert = lo;
+        s.height = height;
+        s.row0 = first_row[lo] + i * height;
+        s.rows = i * height < all ? min(height, all - i * height) : 0u;
+        s.n0 = (2 * nt + rank) * kCh;
+        t += workers;
+        return true;
+    };
+    Strip x;
+    const uint32_t ns = p.steps;
+
+    // Warps 0 to 3 run their loops as whole warps and elect a lane for the asynchronous instructions only (stream.cu).
+    if (warp < kFirstEpi) {
+        ptx::regs_down<kRegsCtrl>();
+        Ring r{0, 0};
+        uint32_t issued = 0, parity = 0;
+        bool ok = true;
+        if (warp == 0) {
+            // ======================= TMA: raw weights =======================
+            const uint32_t blocks = (ns + SPB - 1) / SPB;
+            while (ok && next(x)) {
+                const int y = (int)(x.expert * p.x.n + x.n0);
+                for (uint32_t kb = 0; kb < blocks; ++kb) {
+                    if (!warp_wait(raw_empty(r.i), r.phase ^ 1u, abort_flag)) { give_up(61, x.expert, kb); ok = false; break; }
+                    if (ptx::elect_one()) {
+                        ptx::mbar_arrive_expect_tx(raw_full(r.i), kRawBytes);
+                        ptx::tma_load_2d(smem_base + p.off_raw + r.i * kRawBytes, &tmap_w, (int)(kb * 128u), y, raw_full(r.i));
+                    }
+                    issued |= 1u << r.i; parity = (parity & ~(1u << r.i)) | (r.phase << r.i);
+                    r.step(1, p.raw_stages);
+                }
+            }
+            for (uint32_t s = 0; s < p.raw_stages; ++s)   // never leave with a bulk copy still writing this CTA's shared memory
+                if (issued & (1u << s)) ptx::mbar_wait(raw_full(s), (parity >> s) & 1u);
+        } else if (warp == 1) {
+            // ======================= TMA: rows of A =======================
+            while (ok && next(x)) {
+                const uint32_t act_rows = x.height / 2, slab_bytes = act_rows * 128u;
+                const bool mine = 4u * lane < act_rows;
+                int y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {   // rows behind the last one, and those that A does not have: outside the tensor, zeros
+                    const uint32_t r0 = rank * act_rows + 4u * lane + i;
+                    y[i] = (int)min(mine && r0 < x.rows ? source_row(p.x, x.row0 + r0) : 0xffffffffu, p.x.a_rows);
+                }
+                for (uint32_t l = 0; l < ns; ++l) {
+                    if (!warp_wait(step_empty(r.i), r.phase ^ 1u, abort_flag)) { give_up(62, x.expert, l); ok = false; break; }
+                    if (ptx::elect_one()) ptx::mbar_arrive_expect_tx(step_full(r.i), slab_bytes * (KS / kSlab));
+                    __syncwarp();
+                    if (mine) {
+#pragma unroll
+                        for (int h = 0; h < KS / kSlab; ++h)
+                            ptx::tma_gather4(smem_base + off_act + r.i * act_stride + h * slab_bytes + lane * 512u, &tmap_act, (int)(l * KS + h * kSlab), y[0], y[1], y[2], y[3], step_full(r.i));
+                    }
+                    __syncwarp();
+                    issued |= 1u << r.i; parity = (parity & ~(1u << r.i)) | (r.phase << r.i);
+                    r.step(1, kSlots);
+                }
+            }
+            // nor with a copy on its way, nor while a commit of rank 0 may still arrive here
+            for (uint32_t s = 0; s < kSlots; ++s)
+                if (issued & (1u << s)) (void)warp_wait(step_empty(s), (parity >> s) & 1u, abort_flag);
+            for (uint32_t s = 0; s < kSlots; ++s)
+                if (issued & (1u << s)) ptx::mbar_wait(step_full(s), (parity >> s) & 1u);   // after an abort the converters' part may be missing: then the limit of the wait, far above the time of a copy
+        } else if (rank == 0 && (uint32_t)warp - 2 < kIssuers) {
+            // ======================= MMA issuers: every kIssuers-th step =======================
+            const uint32_t who = (uint32_t)warp - 2;
+            const uint64_t desc0 = ptx::umma_desc_kmajor_sw128(smem_base + off_act);
+            r.i = who;
+            Ring rc{who, 0};
+            bool ready = false;
+            uint32_t before = 0, g = who;   // steps of the tiles walked so far; this warp's next step, counted over all tiles
+            while (ok && next(x)) {
+                const uint32_t idesc = ptx::umma_idesc_bf16_f32(2 * kCh, x.height), slab_d = x.height * 64u >> 4;
+                if (!GROUPED && !warp_wait(acc_empty(rc.i), rc.phase ^ 1u, abort_flag)) { give_up(63, x.expert, 0); break; }
+                for (; g < before + ns; g += kIssuers) {
+                    if (GROUPED && !warp_wait(acc_empty(who), rc.phase ^ 1u, abort_flag)) { give_up(63, x.expert, g); ok = false; break; }
+                    if (!__all_sync(0xffffffffu, ready) && !warp_wait(step_full(r.i), r.phase, abort_flag)) { give_up(64, x.expert, g); ok = false; break; }
+                    ptx::tc_fence_after_sync();
+                    const uint32_t ta = slot_base + r.i * kSlotCols, td = tmem_base + rc.i * acc_cols, done = step_empty(r.i), acc_done = acc_full(rc.i);
+                    const uint64_t db = desc0 + r.i * (act_stride >> 4);
+                    const bool first = GROUPED || g == before, last = GROUPED || g + 1 == before + ns;
+                    r.step(kIssuers, kSlots);
+                    ready = ptx::mbar_test_wait(step_full(r.i), r.phase);   // of the next step: the answer is back when this one has been issued
+                    if (ptx::elect_one()) {
+#pragma unroll
+                        for (int j = 0; j < KS / 16; ++j)
+                            ptx::umma_bf16_ts_pair(td, ta + 8 * j, db + (uint32_t)(j / 4) * slab_d + 2u * (j % 4), idesc, !first || j > 0 ? 1u : 0u);
+                        ptx::umma_commit_pair(done);
+                        if (last) ptx::umma_commit_pair(acc_done);
+                    }
+                    if (GROUPED) rc.phase ^= 1u;
+                }
+                before += ns;
+                if (!GROUPED) rc.step(1, p.accs);
+            }
+        } else if (warp == 2) {
+            // ======================= rank 1: reports its half of each step =======================
+            while (ok && next(x)) {
+                for (uint32_t l = 0; l < ns; ++l) {
+                    if (!warp_wait(step_full(r.i), r.phase, abort_flag)) { give_up(65, x.expert, l); ok = false; break; }
+                    ptx::tc_fence_after_sync();
+                    ptx::tc_fence_before_sync();
+                    if (ptx::elect_one()) ptx::mbar_arrive_remote(step_full(r.i), 0);
+                    r.step(1, kSlots);
+                }
+            }
+        }
+    } else if (warp >= kFirstConv) {
+        // ======================= converters =======================
+        ptx::regs_down<kRegsConv>();
+        const uint32_t g = (uint32_t)(warp - kFirstConv) >> 2, quarter = (uint32_t)warp & 3u;
+        const uint32_t ch = quarter * 32 + lane;
+        const uint32_t flip = BITS == 8 ? flip8(p.x.enc) : flip4(p.x.enc);
+        const uint32_t sel0 = p.x.packed ? kSel8Strided02 : kSel8Natural01, sel1 = p.x.packed ? kSel8Strided13 : kSel8Natural23;
+        const Nibbles nib = nibbles(p.x.packed != 0);
+        const bool has_zero = p.x.zero != nullptr;
+        const uint32_t groups_per_row = GROUPED ? p.x.k >> p.x.group_shift : 0;
+        auto zero_add = [&](size_t i) { return unpack_add(BITS, BITS == 8 ? decode_zero8(p.x.zero[i], p.x.enc) : decode_zero4(p.x.zero[i], p.x.enc)); };
+        uint32_t add = unpack_add(BITS, 0);
+        const uint32_t row = p.off_raw + ch * 128, swz = (ch & 7u) << 4, lanes = (quarter * 32u) << 16;
+        uint32_t steps_before = 0, blocks_before = 0;   // of the tiles walked so far
+        bool ok = true;
+        while (ok && next(x)) {
+            const uint32_t nn = x.n0 + ch;
+            const size_t chan = (size_t)x.expert * p.x.n + (nn < p.x.n ? nn : 0);
+            if (!GROUPED && has_zero) add = zero_add(chan);
+            uint32_t l = (g - steps_before) & (kGroups - 1);
+            Ring rr, rs;
+            rr.set(blocks_before + l / SPB, p.raw_stages);
+            rs.set(steps_before + l, kSlots);
+            for (; l < ns; l += kGroups) {
+                const uint32_t sub = l % SPB;
+                if (GROUPED && has_zero) add = zero_add(chan * groups_per_row + ((l * KS) >> p.x.group_shift));
+                if (p.slot_first && !warp_wait(step_empty(rs.i), rs.phase ^ 1u, abort_flag)) { give_up(66, x.expert, l); ok = false; break; }
+                if (!warp_wait(raw_full(rr.i), rr.phase, abort_flag)) { give_up(67, x.expert, l); ok = false; break; }
+                const uint32_t raw = smem_base + row + rr.i * kRawBytes, slot = slot_base + lanes + rs.i * kSlotCols;
+                // KS / 64 times: the raw words of 64 k (of int4 the whole step's) first, then 32 k at a time
+                constexpr int kWords = BITS == 8 ? 16 : KS / 8, kPieces = BITS == 8 ? KS / 64 : 1, kPerStore = BITS == 8 ? 8 : 4;
+#pragma unroll
+                for (int h = 0; h < kPieces; ++h) {
+                    uint32_t w[kWords];
+#pragma unroll
+                    for (int i = 0; i < kWords / 4; ++i) {
+                        const uint32_t at = raw + ((((sub * kPieces + h) * (kWords / 4) + i) << 4) ^ swz);
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3]) : "r"(at));
+                    }
+#pragma unroll
+                    for (int q = 0; q < kWords / kPerStore; ++q) {
+                        uint32_t o[16];
+#pragma unroll
+                        for (int j = 0; j < kPerStore; ++j) {
+                            const uint32_t v = w[q * kPerStore + j];
+                            if (BITS == 8) {
+                                s8x4_to_bf16(v, flip, sel0, sel1, kMulByte, add, o[2 * j], o[2 * j + 1]);
+                            } else {
+                                uint32_t qv[4];
+                                s4x8_to_bf16(v, flip, nib, nib.mul[0], nib.mul[1], add, qv);
+                                o[4 * j] = qv[0]; o[4 * j + 1] = qv[1]; o[4 * j + 2] = qv[2]; o[4 * j + 3] = qv[3];
+                            }
+                        }
+                        if (h == 0 && q == 0) {
+                            if (!p.slot_first && !warp_wait(step_empty(rs.i), rs.phase ^ 1u, abort_flag)) { give_up(66, x.expert, l); ok = false; break; }
+                            ptx::tc_fence_after_sync();
+                        }
+                        ptx::tmem_st_32x16(slot + (h * (kWords / kPerStore) + q) * 16, o);
+                    }
+                    if (!ok) break;
+                }
+                if (!ok) break;
+                ptx::tmem_st_wait();
+                ptx::tc_fence_before_sync();
+                __syncwarp();   // every lane's weights are in tensor memory
+                if (lane == 0) {
+                    ptx::mbar_arrive(step_full(rs.i));
+                    const uint32_t left = ns - (l - sub);   // steps of this block and all after it
+                    ptx::mbar_arrive_count(raw_empty(rr.i), left < SPB && sub + 1 == left ? 1 + SPB - left : 1u);   // a short last block: for its missing steps, too
+                }
+                rr.step(kGroups / SPB, p.raw_stages);   // four steps on
+                rs.step(kGroups, kSlots);
+            }
+            steps_before += ns;
+            blocks_before += (ns + SPB - 1) / SPB;
+        }
+    } else {
+        // ======================= epilogue =======================
+        ptx::regs_up<kRegsEpi>();
+        const uint32_t quarter = (uint32_t)warp & 3u, half = (uint32_t)(warp - kFirstEpi) >> 2, ch = quarter * 32 + lane;
+        constexpr int kPacks = GROUPED ? 4 : 8;   // of 16 columns: this warp's half of a strip
+        const bool odd = lane & 1, gated = p.x.gated != 0, act = p.x.silu != 0;
+        const uint32_t stage = smem_base + kOffOut + (uint32_t)(warp - kFirstEpi) * 2 * kOutBytes;
+        const uint32_t groups_per_row = GROUPED ? p.x.k >> p.x.group_shift : 0;
+        Ring rc{0, 0};
+        bool ok = true;
+        auto drained = [&] {   // everything of the accumulator is in registers
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) { if (rank == 0) ptx::mbar_arrive(acc_empty(rc.i)); else ptx::mbar_arrive_remote(acc_empty(rc.i), 0); }
+        };
+        auto pack2 = [](float lo, float hi) {
+            const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+            return *reinterpret_cast<const uint32_t*>(&v);
+        };
+        auto put = [&](uint32_t at, uint32_t v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"((uint16_t)v) : "memory"); };
+        while (ok && next(x)) {
+            const uint32_t cols = x.height / 2, nn = x.n0 + ch;
+            const size_t chan = (size_t)x.expert * p.x.n + (nn < p.x.n ? nn : 0);
+            // 16 finished sums of this lane's channel -> packed results.  Gated: the lanes of a pair hold gate (even) and up (odd) of one output
+            // channel and exchange half of the 16 rows: the even lane finishes rows 0 to 7, the odd one 8 to 15.
+            uint32_t o[kPacks][8];
+            auto finish = [&](uint32_t (&to)[8], const float (&v)[16]) {
+                if (gated) {
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) {
+                        float f[2];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float lo = v[j + i], hi = v[j + i + 8], other = __shfl_xor_sync(0xffffffffu, odd ? lo : hi, 1);
+                            const float gate = odd ? other : lo, up = odd ? hi : other;
+                            f[i] = (act ? silu(gate) : gate) * up;
+                        }
+                        to[j / 2] = pack2(f[0], f[1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) to[j] = pack2(act ? silu(v[2 * j]) : v[2 * j], act ? silu(v[2 * j + 1]) : v[2 * j + 1]);
+                }
+            };
+            const uint32_t column = tmem_base + ((quarter * 32u) << 16) + half * cols;
+            if (GROUPED) {
+                float sum[kPacks][16];
+#pragma unroll
+                for (int i = 0; i < kPacks; ++i)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) sum[i][j] = 0.f;
+                auto group_scale = [&](uint32_t l) {
+                    if (l >= ns) return 0.f;
+                    const size_t i = chan * groups_per_row + ((l * KS) >> p.x.group_shift);
+                    return p.x.scale_dtype == AFB_SCALE_BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.x.scale)[i] << 16)
+                                                             : reinterpret_cast<const float*>(p.x.scale)[i];
+                };
+                float sc = group_scale(0);
+                for (uint32_t l = 0; l < ns; ++l) {
+                    const float sc_nxt = group_scale(l + 1);
+                    if (!warp_wait(acc_full(rc.i), rc.phase, abort_flag)) { give_up(68, x.expert, l); ok = false; break; }
+                    ptx::tc_fence_after_sync();
+#pragma unroll
+                    for (int i = 0; i < kPacks; i += 2) {
+                        if (16u * i >= cols) break;
+                        uint32_t a[16], b[16];
+                        ptx::tmem_ld_32x16(column + rc.i * acc_cols + 16 * i, a);
+                        if (16u * (i + 1) < cols) ptx::tmem_ld_32x16(column + rc.i * acc_cols + 16 * (i + 1), b);
+                        ptx::tmem_ld_wait();
+                        if (16u * (i + 2) >= cols) drained();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) sum[i][j] = fmaf(sc, __uint_as_float(a[j]), sum[i][j]);
+                        if (16u * (i + 1) < cols) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) sum[i + 1][j] = fmaf(sc, __uint_as_float(b[j]), sum[i + 1][j]);
+                        }
+                    }
+                    rc.step(1, 2);
+                    sc = sc_nxt;
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < kPacks; ++i) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) sum[i][j] *= kUnpackInverse;
+                    finish(o[i], sum[i]);
+                }
+            } else {
+                const float scale = p.x.scale_dtype == AFB_SCALE_BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.x.scale)[chan] << 16)
+                                                                      : reinterpret_cast<const float*>(p.x.scale)[chan];
+                if (!warp_wait(acc_full(rc.i), rc.phase, abort_flag)) { give_up(68, x.expert, 0); break; }
+                ptx::tc_fence_after_sync();
+#pragma unroll
+                for (int i = 0; i < kPacks; ++i) {
+                    if (16u * i >= cols) break;
+                    uint32_t a[16];
+                    float v[16];
+                    ptx::tmem_ld_32x16(column + rc.i * acc_cols + 16 * i, a);
+                    ptx::tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] = unscaled(__uint_as_float(a[j]), scale);
+                    finish(o[i], v);
+                }
+                drained();
+                rc.step(1, p.accs);
+            }
+            // Blocks of 16 rows turn round in shared memory and leave in 16-byte pieces, 64 (gated 32) contiguous bytes a row; two blocks take turns.
+            const uint32_t first = half * cols, valid = x.rows > first ? min(cols, x.rows - first) : 0u;
+            const uint32_t c0 = x.n0 + quarter * 32u;   // first channel of this warp
+            if (c0 >= p.x.n) continue;
+            uint16_t* c = p.x.c + (size_t)(x.row0 + first) * p.x.ldc;
+#pragma unroll
+            for (int i = 0; i < kPacks; ++i) {
+                if (16u * i >= valid) break;
+                if (p.c_vec) {
+                    const uint32_t out = stage + (i & 1) * kOutBytes;
+                    if (gated) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t at = out + ((odd ? 8u : 0u) + 2 * j) * 32u + ((uint32_t)lane >> 1) * 2u;
+                            put(at, o[i][j]); put(at + 32u, o[i][j] >> 16);
+                        }
+                        __syncwarp();
+                        const uint32_t row = 16u * i + lane / 2, col = c0 / 2 + (lane & 1) * 8;
+                        uint4 v;
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(out + lane * 16u));
+                        if (row < valid && col < p.x.n_out) *reinterpret_cast<uint4*>(c + (size_t)row * p.x.ldc + col) = v;   // n_out is a multiple of 8
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const uint32_t at = out + (uint32_t)j * 128u + (uint32_t)lane * 2u;
+                            put(at, o[i][j]); put(at + 64u, o[i][j] >> 16);
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (uint32_t h = 0; h < 2; ++h) {
+                            const uint32_t piece = h * 32 + lane, row = 16u * i + piece / 4, col = c0 + piece % 4 * 8;
+                            uint4 v;
+                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(out + piece * 16));
+                            if (row < valid && col < p.x.n_out) *reinterpret_cast<uint4*>(c + (size_t)row * p.x.ldc + col) = v;
+                        }
+                    }
+                } else if (gated) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t row = 16u * i + (odd ? 8u : 0u) + j;
+                        if (row < valid && nn < p.x.n) c[(size_t)row * p.x.ldc + nn / 2] = (uint16_t)(o[i][j / 2] >> (j % 2 * 16));
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (16u * i + j < valid && nn < p.x.n) c[(size_t)(16u * i + j) * p.x.ldc + nn] = (uint16_t)(o[i][j / 2] >> (j % 2 * 16));
+                }
+            }
+            __syncwarp();   // the next tile's first block is written after this one's last has been read
+        }
+    }
+
+    // ---- teardown: every thread gets here, also after an abort; neither CTA leaves while the other may read its shared memory or arrive there ----
+    ptx::tc_fence_before_sync();
+    __syncwarp();
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+    if (warp == 2) {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc_pair(tmem_base, kTmemCols);
+    }
+}
+
+template <int BITS, bool GROUPED, int KS>
+int launch_cfg(const CUtensorMap& ta, const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uint32_t smem, DeviceCtx* ctx, cudaStream_t s) {
+    auto kern = expert_many_kernel<BITS, GROUPED, KS>;
+    static DeviceOnce attr_set;  // per template instance
+    if (!attr_set.done(ctx->device)) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+        if (e != cudaSuccess) return cuda_fail(e);
+        attr_set.mark(ctx->device);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(kManyThreads); cfg.stream = s; cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tw, p);
+    count_launch();
+    return e == cudaSuccess ? AFB_OK : cuda_fail(e);
+}
+
+}  // namespace
+
+int launch_expert_many(const ExpertParams& q, uint32_t bits, uint32_t group, DeviceCtx* ctx, cudaStream_t s) {
+    ManyParams p{};
+    p.x = q;
+    const uint32_t ks = q.k % 128 == 0 && group % 128 == 0 ? 128 : 64, spb = (bits == 8 ? 128 : 256) / ks, kSlots = slots(ks);
+    // up to 128 rows there are two accumulators, and twice the raw blocks under way
+    p.x.tile_rows = group || (uint64_t)q.m <= 160ull * q.experts ? 128 : 256;
+    p.x.n_blocks = (q.n + 2 * kCh - 1) / (2 * kCh);
+    p.steps = q.k / ks;
+    p.accs = p.x.tile_rows <= 128 ? 2 : 1;
+    p.off_raw = (kOffTable + (3 * q.experts + 1) * (uint32_t)sizeof(uint32_t) + 1023u) / 1024u * 1024u;
+    const uint32_t act_bytes = kSlots * p.x.tile_rows * ks;
+    p.raw_stages = (232448 - 1024 - p.off_raw - act_bytes) / kRawBytes;
+    if (p.raw_stages > (uint32_t)kMaxRaw) p.raw_stages = kMaxRaw;
+    // The parity waits of the converters (stream.cu): a converter warp sees every fourth step only, and its wait for phase n of a raw block means
+    // something once phase n - 1 is complete.  A free slot says that the step kSlots back has been multiplied and so, with one issuing warp, all
+    // before it.  With two, the other one may be a step behind: its last but one has been, since the accumulators are drained in order.
+    const uint32_t back = kSlots + (group ? 2 : 0), per_block = p.steps % spb == 0 ? spb : 1;
+    p.slot_first = p.raw_stages * per_block >= kGroups + back + per_block - 1 ? 0u : 1u;
+    if (p.raw_stages * per_block < back + per_block - 1) return AFB_ERR_UNSUPPORTED;   // not with any size that this function takes
+    p.c_vec = q.ldc % 8 == 0 && (uintptr_t)q.c % 16 == 0 && q.n_out % 8 == 0;
+    p.status = ctx->status;
+    const uint64_t tiles = expert_tiles(q.m, q.experts, p.x.tile_rows) * p.x.n_blocks;
+    if (tiles >> 31) return AFB_ERR_TOO_LARGE;
+    const uint32_t pairs = (uint32_t)ctx->sm_count / 2, grid = 2 * (tiles < pairs ? (uint32_t)tiles : pairs);
+    const uint32_t smem = 1024 + p.off_raw + p.raw_stages * kRawBytes + act_bytes;
+    CUtensorMap ta, tw;
+    int rc = tmap_2d(&ta, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, q.a, q.k, q.a_rows, (uint64_t)q.lda * 2, kSlab, 1, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+    rc = tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.b, (uint64_t)q.k * bits / 8, (uint64_t)q.experts * q.n, q.ldb_bytes, 128, kCh, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+    if (bits == 4 && !group) return launch_cfg<4, false, 128>(ta, tw, p, grid, smem, ctx, s);   // k is a multiple of 128
+    if (bits == 4) return ks == 128 ? launch_cfg<4, true, 128>(ta, tw, p, grid, smem, ctx, s) : launch_cfg<4, true, 64>(ta, tw, p, grid, smem, ctx, s);
+    if (group) return ks == 128 ? launch_cfg<8, true, 128>(ta, tw, p, grid, smem, ctx, s) : launch_cfg<8, true, 64>(ta, tw, p, grid, smem, ctx, s);
+    return ks == 128 ? launch_cfg<8, false, 128>(ta, tw, p, grid, smem, ctx, s) : launch_cfg<8, false, 64>(ta, tw, p, grid, smem, ctx, s);
+}
+
+}  // namespace afb
