@@ -6,10 +6,11 @@
 // one tcgen05.mma.cta_group::2 reads both halves.  An expert's rows are cut into strips of equal height, a multiple of 32.
 //
 //   warp 0        TMA: raw weight blocks, 128 channels x 128 bytes, 128-byte swizzle
-//   warp 1        TMA gather of this CTA's half of the strip: four rows of 64 k per instruction and lane, 128-byte swizzle
 //   warps 2, 3    rank 0: tcgen05.mma 256 x height x 16;  rank 1, warp 2: reports to rank 0 that its half of a step is complete
 //   warps 4-11    epilogue, two per lane quarter: accumulator -> registers -> (accumulator free) -> shared memory -> C
 //   warps 12-27   converters: four groups of four warps; group g takes every fourth step of k (KS = 128 or 64 wide)
+//   warps 28-31   the rows of A: 16-byte copies to shared memory, written in the 128-byte swizzle.  (A TMA gather of four rows takes 65 cycles of
+//                 the issuing warp, which has to make every lane's row numbers uniform first: 4200 cycles per step of 256 rows.)
 //
 // Scales per channel: the sum over all of K stays in the accumulator, strips of up to 256 rows.
 // Scales per group: a weight times its scale has no room in a bf16 (up to 8 x 8 significant bits), and rounding it there costs as much
@@ -26,10 +27,10 @@
 namespace afb {
 namespace {
 
-constexpr int kFirstEpi = 4, kEpiWarps = 8, kFirstConv = kFirstEpi + kEpiWarps;
-constexpr int kManyThreads = 32 * (kFirstConv + 4 * kGroups);   // 896: launched with 72 registers a thread
-constexpr uint32_t kRegsCtrl = 56, kRegsEpi = 112, kRegsConv = 56;
-static_assert(128 * kRegsCtrl + 32 * kEpiWarps * kRegsEpi + 128 * kGroups * kRegsConv <= 72 * kManyThreads, "shares of the registers");
+constexpr int kFirstEpi = 4, kEpiWarps = 8, kFirstConv = kFirstEpi + kEpiWarps, kFirstLoad = kFirstConv + 4 * kGroups, kLoadWarps = 4;
+constexpr int kManyThreads = 32 * (kFirstLoad + kLoadWarps);   // 1024: launched with 64 registers a thread
+constexpr uint32_t kRegsCtrl = 40, kRegsEpi = 104, kRegsConv = 56, kRegsLoad = 40;
+static_assert(128 * kRegsCtrl + 32 * kEpiWarps * kRegsEpi + 128 * kGroups * kRegsConv + 32 * kLoadWarps * kRegsLoad <= 64 * kManyThreads, "shares of the registers");
 constexpr int kMaxRaw = 12, kMaxSlots = 8, kMaxAcc = 2;
 __host__ __device__ constexpr uint32_t slots(int ks) { return ks == 128 ? 4 : 6; }   // steps under way, in 256 columns at most
 constexpr uint32_t kTmemCols = 512;
@@ -50,11 +51,18 @@ struct ManyParams {
     int32_t* status;
 };
 
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void cp_async_wait_but2() { asm volatile("cp.async.wait_group 2;" ::: "memory"); }
+
 struct Strip { uint32_t expert, row0, rows, height, n0; };   // n0: of this CTA's 128 channels
 
 template <int BITS, bool GROUPED, int KS>
 __global__ void __launch_bounds__(kManyThreads, 1)
-expert_many_kernel(const __grid_constant__ CUtensorMap tmap_act, const __grid_constant__ CUtensorMap tmap_w, const ManyParams p) {
+expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams p) {
     constexpr uint32_t SPB = (BITS == 8 ? 128 : 256) / KS;   // steps per raw block
     constexpr uint32_t kSlotCols = KS / 2;                   // TMEM columns of a step's weights
     constexpr uint32_t kSlots = slots(KS);
@@ -82,11 +90,10 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_act, const __grid_co
 
     if (warp == 0 && lane == 0) {
         for (uint32_t s = 0; s < p.raw_stages; ++s) { ptx::mbar_init(raw_full(s), 1); ptx::mbar_init(raw_empty(s), 4 * SPB); }
-        for (uint32_t s = 0; s < kSlots; ++s) { ptx::mbar_init(step_full(s), 4 + 1 + (rank == 0 ? 1 : 0)); ptx::mbar_init(step_empty(s), 1); }
+        for (uint32_t s = 0; s < kSlots; ++s) { ptx::mbar_init(step_full(s), 4 + kLoadWarps + (rank == 0 ? 1 : 0)); ptx::mbar_init(step_empty(s), 1); }
         for (uint32_t s = 0; s < p.accs; ++s) { ptx::mbar_init(acc_full(s), 1); ptx::mbar_init(acc_empty(s), 2 * kEpiWarps); }
         *abort_flag = 0;
         ptx::fence_mbar_init();
-        ptx::prefetch_tmap(&tmap_act);
         ptx::prefetch_tmap(&tmap_w);
     }
     if (warp == 2) {
@@ -173,36 +180,6 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_act, const __grid_co
             }
             for (uint32_t s = 0; s < p.raw_stages; ++s)   // never leave with a bulk copy still writing this CTA's shared memory
                 if (issued & (1u << s)) ptx::mbar_wait(raw_full(s), (parity >> s) & 1u);
-        } else if (warp == 1) {
-            // ======================= TMA: rows of A =======================
-            while (ok && next(x)) {
-                const uint32_t act_rows = x.height / 2, slab_bytes = act_rows * 128u;
-                const bool mine = 4u * lane < act_rows;
-                int y[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {   // rows behind the last one, and those that A does not have: outside the tensor, zeros
-                    const uint32_t r0 = rank * act_rows + 4u * lane + i;
-                    y[i] = (int)min(mine && r0 < x.rows ? source_row(p.x, x.row0 + r0) : 0xffffffffu, p.x.a_rows);
-                }
-                for (uint32_t l = 0; l < ns; ++l) {
-                    if (!warp_wait(step_empty(r.i), r.phase ^ 1u, abort_flag)) { give_up(62, x.expert, l); ok = false; break; }
-                    if (ptx::elect_one()) ptx::mbar_arrive_expect_tx(step_full(r.i), slab_bytes * (KS / kSlab));
-                    __syncwarp();
-                    if (mine) {
-#pragma unroll
-                        for (int h = 0; h < KS / kSlab; ++h)
-                            ptx::tma_gather4(smem_base + off_act + r.i * act_stride + h * slab_bytes + lane * 512u, &tmap_act, (int)(l * KS + h * kSlab), y[0], y[1], y[2], y[3], step_full(r.i));
-                    }
-                    __syncwarp();
-                    issued |= 1u << r.i; parity = (parity & ~(1u << r.i)) | (r.phase << r.i);
-                    r.step(1, kSlots);
-                }
-            }
-            // nor with a copy on its way, nor while a commit of rank 0 may still arrive here
-            for (uint32_t s = 0; s < kSlots; ++s)
-                if (issued & (1u << s)) (void)warp_wait(step_empty(s), (parity >> s) & 1u, abort_flag);
-            for (uint32_t s = 0; s < kSlots; ++s)
-                if (issued & (1u << s)) ptx::mbar_wait(step_full(s), (parity >> s) & 1u);   // after an abort the converters' part may be missing: then the limit of the wait, far above the time of a copy
         } else if (rank == 0 && (uint32_t)warp - 2 < kIssuers) {
             // ======================= MMA issuers: every kIssuers-th step =======================
             const uint32_t who = (uint32_t)warp - 2;
@@ -247,7 +224,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_act, const __grid_co
                 }
             }
         }
-    } else if (warp >= kFirstConv) {
+    } else if (warp >= kFirstConv && warp < kFirstLoad) {
         // ======================= converters =======================
         ptx::regs_down<kRegsConv>();
         const uint32_t g = (uint32_t)(warp - kFirstConv) >> 2, quarter = (uint32_t)warp & 3u;
@@ -323,6 +300,57 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_act, const __grid_co
             steps_before += ns;
             blocks_before += (ns + SPB - 1) / SPB;
         }
+    } else if (warp >= kFirstLoad) {
+        // ======================= rows of A =======================
+        // A lane copies 16 bytes of rows 16 * i + 4 * (which loader) + lane / 8 of this CTA's half, per 64 k.
+        ptx::regs_down<kRegsLoad>();
+        const uint32_t r8 = (uint32_t)(warp - kFirstLoad) * 4 + ((uint32_t)lane >> 3), piece = (uint32_t)lane & 7u;
+        const uint32_t at = smem_base + off_act + r8 * 128u + ((piece ^ (r8 & 7u)) << 4);   // 16 rows on: the same place in the swizzle
+        Ring r{0, 0}, rp{0, 0};       // of the step that comes next, of the oldest one that has not been reported
+        uint32_t pending = 0, issued = 0, parity = 0;
+        bool ok = true;
+        // The copies are this thread's writes; tcgen05.mma reads shared memory through the asynchronous proxy.
+        auto report = [&] {
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(step_full(rp.i));
+            rp.step(1, kSlots);
+            --pending;
+        };
+        while (ok && next(x)) {
+            const uint32_t act_rows = x.height / 2, slab_bytes = act_rows * 128u;   // act_rows: a multiple of 16
+            const uint16_t* src[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {   // rows behind the last one, and those that A does not have: zeros
+                const uint32_t r0 = 16u * i + r8, c = rank * act_rows + r0;
+                const uint32_t row = r0 < act_rows && c < x.rows ? source_row(p.x, x.row0 + c) : 0xffffffffu;
+                src[i] = row < p.x.a_rows ? p.x.a + (size_t)row * p.x.lda + piece * 8u : nullptr;
+            }
+            for (uint32_t l = 0; l < ns; ++l) {
+                // a free slot: go on; otherwise first report all that is under way
+                if (!__all_sync(0xffffffffu, ptx::mbar_test_wait(step_empty(r.i), r.phase ^ 1u))) {
+                    if (pending) { cp_async_wait_all(); while (pending) report(); }
+                    if (!warp_wait(step_empty(r.i), r.phase ^ 1u, abort_flag)) { give_up(62, x.expert, l); ok = false; break; }
+                }
+                const uint32_t to = at + r.i * act_stride;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (16u * i >= act_rows) break;
+#pragma unroll
+                    for (int h = 0; h < KS / kSlab; ++h)
+                        cp_async16_or_zero(to + h * slab_bytes + i * 2048u, src[i] ? (const void*)(src[i] + (size_t)l * KS + h * kSlab) : (const void*)p.x.a, src[i] != nullptr);
+                }
+                cp_async_commit();
+                ++pending;
+                issued |= 1u << r.i; parity = (parity & ~(1u << r.i)) | (r.phase << r.i);
+                r.step(1, kSlots);
+                if (pending > 2) { cp_async_wait_but2(); report(); }
+            }
+        }
+        cp_async_wait_all();
+        while (pending) report();
+        for (uint32_t s = 0; s < kSlots; ++s)   // not while a commit of rank 0 may still arrive here
+            if (issued & (1u << s)) (void)warp_wait(step_empty(s), (parity >> s) & 1u, abort_flag);
     } else {
         // ======================= epilogue =======================
         ptx::regs_up<kRegsEpi>();
@@ -386,19 +414,14 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_act, const __grid_co
                     if (!warp_wait(acc_full(rc.i), rc.phase, abort_flag)) { give_up(68, x.expert, l); ok = false; break; }
                     ptx::tc_fence_after_sync();
 #pragma unroll
-                    for (int i = 0; i < kPacks; i += 2) {
+                    for (int i = 0; i < kPacks; ++i) {
                         if (16u * i >= cols) break;
-                        uint32_t a[16], b[16];
+                        uint32_t a[16];
                         ptx::tmem_ld_32x16(column + rc.i * acc_cols + 16 * i, a);
-                        if (16u * (i + 1) < cols) ptx::tmem_ld_32x16(column + rc.i * acc_cols + 16 * (i + 1), b);
                         ptx::tmem_ld_wait();
-                        if (16u * (i + 2) >= cols) drained();
+                        if (16u * (i + 1) >= cols) drained();
 #pragma unroll
                         for (int j = 0; j < 16; ++j) sum[i][j] = fmaf(sc, __uint_as_float(a[j]), sum[i][j]);
-                        if (16u * (i + 1) < cols) {
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) sum[i + 1][j] = fmaf(sc, __uint_as_float(b[j]), sum[i + 1][j]);
-                        }
                     }
                     rc.step(1, 2);
                     sc = sc_nxt;
@@ -493,7 +516,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_act, const __grid_co
 }
 
 template <int BITS, bool GROUPED, int KS>
-int launch_cfg(const CUtensorMap& ta, const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uint32_t smem, DeviceCtx* ctx, cudaStream_t s) {
+int launch_cfg(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uint32_t smem, DeviceCtx* ctx, cudaStream_t s) {
     auto kern = expert_many_kernel<BITS, GROUPED, KS>;
     static DeviceOnce attr_set;  // per template instance
     if (!attr_set.done(ctx->device)) {
@@ -507,7 +530,7 @@ int launch_cfg(const CUtensorMap& ta, const CUtensorMap& tw, const ManyParams& p
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, ta, tw, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, p);
     count_launch();
     return e == cudaSuccess ? AFB_OK : cuda_fail(e);
 }
@@ -539,15 +562,13 @@ int launch_expert_many(const ExpertParams& q, uint32_t bits, uint32_t group, Dev
     if (tiles >> 31) return AFB_ERR_TOO_LARGE;
     const uint32_t pairs = (uint32_t)ctx->sm_count / 2, grid = 2 * (tiles < pairs ? (uint32_t)tiles : pairs);
     const uint32_t smem = 1024 + p.off_raw + p.raw_stages * kRawBytes + act_bytes;
-    CUtensorMap ta, tw;
-    int rc = tmap_2d(&ta, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, q.a, q.k, q.a_rows, (uint64_t)q.lda * 2, kSlab, 1, CU_TENSOR_MAP_SWIZZLE_128B);
+    CUtensorMap tw;
+    const int rc = tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.b, (uint64_t)q.k * bits / 8, (uint64_t)q.experts * q.n, q.ldb_bytes, 128, kCh, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
-    rc = tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.b, (uint64_t)q.k * bits / 8, (uint64_t)q.experts * q.n, q.ldb_bytes, 128, kCh, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc) return rc;
-    if (bits == 4 && !group) return launch_cfg<4, false, 128>(ta, tw, p, grid, smem, ctx, s);   // k is a multiple of 128
-    if (bits == 4) return ks == 128 ? launch_cfg<4, true, 128>(ta, tw, p, grid, smem, ctx, s) : launch_cfg<4, true, 64>(ta, tw, p, grid, smem, ctx, s);
-    if (group) return ks == 128 ? launch_cfg<8, true, 128>(ta, tw, p, grid, smem, ctx, s) : launch_cfg<8, true, 64>(ta, tw, p, grid, smem, ctx, s);
-    return ks == 128 ? launch_cfg<8, false, 128>(ta, tw, p, grid, smem, ctx, s) : launch_cfg<8, false, 64>(ta, tw, p, grid, smem, ctx, s);
+    if (bits == 4 && !group) return launch_cfg<4, false, 128>(tw, p, grid, smem, ctx, s);   // k is a multiple of 128
+    if (bits == 4) return ks == 128 ? launch_cfg<4, true, 128>(tw, p, grid, smem, ctx, s) : launch_cfg<4, true, 64>(tw, p, grid, smem, ctx, s);
+    if (group) return ks == 128 ? launch_cfg<8, true, 128>(tw, p, grid, smem, ctx, s) : launch_cfg<8, true, 64>(tw, p, grid, smem, ctx, s);
+    return ks == 128 ? launch_cfg<8, false, 128>(tw, p, grid, smem, ctx, s) : launch_cfg<8, false, 64>(tw, p, grid, smem, ctx, s);
 }
 
 }  // namespace afb

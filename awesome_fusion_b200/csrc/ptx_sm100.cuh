@@ -86,13 +86,6 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* m, 
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y) : "memory");
 }
 
-// Four rows of a 2-D tensor, each `box` wide (the map's box is one row high): x as above, a row outside the tensor reads as zeros.
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* m, int x, int y0, int y1, int y2, int y3, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y0), "r"(y1), "r"(y2), "r"(y3) : "memory");
-}
-
 // Tile store shared -> global (bulk async-group completion).  The writes to shared memory that precede it must have been made
 // visible to the async proxy (fence_proxy_async_smem) by the threads that wrote them.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* m, uint32_t src, int x, int y) {
