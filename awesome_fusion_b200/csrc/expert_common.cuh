@@ -1,5 +1,5 @@
-// Shared by the two forms of the products grouped by expert (expert_few.cu, expert_many.cu): the parameter block and the way a CTA finds its
-// tile.  How many rows an expert has is known on the GPU only; the launch covers the most tiles there can be, the rest find nothing to do.
+// Shared by the two forms of the products grouped by expert (expert_few.cu, expert_many.cu): the parameter block and the table by which a CTA
+// finds its tiles.  How many rows an expert has is known on the GPU only.
 #pragma once
 #include "activation.cuh"
 #include "afb_internal.h"
@@ -29,44 +29,58 @@ inline uint64_t expert_tiles(uint32_t m, uint32_t experts, uint32_t rows) {
     return active + (uint64_t)(m - active) / rows;
 }
 
-struct ExpertTile { uint32_t expert, row0, rows, tiles_before; };
-
 __device__ __forceinline__ uint32_t clamp_offset(int32_t o, uint32_t m) { return (uint32_t)min(max(o, 0), (int32_t)m); }
 
-// Tile number `slot` in the order of the experts, by a whole warp; false: there are fewer.  An expert's rows are cut into as few tiles as
-// fit, of equal height but for the last; `unit` rounds the height up.
-__device__ __forceinline__ bool find_tile(const ExpertParams& p, uint32_t slot, uint32_t unit, uint32_t lane, ExpertTile& x) {
-    uint32_t before = 0;
-    for (uint32_t e0 = 0; e0 < p.experts; e0 += 32) {
-        const uint32_t e = e0 + lane;
-        uint32_t lo = 0, hi = 0;
-        if (e < p.experts) {
-            lo = clamp_offset(__ldg(p.offsets + e), p.m);
-            hi = max(lo, clamp_offset(__ldg(p.offsets + e + 1), p.m));
-        }
-        const uint32_t rows = hi - lo, tiles = (rows + p.tile_rows - 1) / p.tile_rows;
-        uint32_t upto = tiles;
+// One tile: rows [row0, row0 + rows) of an expert, at most `height` of them, x channel block `block`.
+struct ExpertStrip { uint32_t expert, row0, rows, height, block; };
+
+// Where each expert's rows and strips (its rows cut into as few as fit tile_rows, of equal height but for the last) begin, in shared memory.
+struct ExpertTable {
+    uint32_t *strips_before, *first_row, *row_count;   // [experts + 1], [experts], [experts]
+    uint32_t experts;
+    __host__ __device__ static uint32_t bytes(uint32_t experts) { return (3 * experts + 1) * (uint32_t)sizeof(uint32_t); }
+    __device__ __forceinline__ ExpertTable(void* at, uint32_t n)
+        : strips_before(reinterpret_cast<uint32_t*>(at)), first_row(strips_before + n + 1), row_count(first_row + n), experts(n) {}
+    __device__ __forceinline__ uint32_t strips() const { return strips_before[experts]; }
+    // By one warp, before a barrier of all.
+    __device__ __forceinline__ void build(const ExpertParams& p, uint32_t lane) const {
+        uint32_t before = 0;
+        for (uint32_t e0 = 0; e0 < experts; e0 += 32) {
+            const uint32_t e = e0 + lane;
+            uint32_t lo = 0, hi = 0;
+            if (e < experts) {
+                lo = clamp_offset(__ldg(p.offsets + e), p.m);
+                hi = max(lo, clamp_offset(__ldg(p.offsets + e + 1), p.m));
+            }
+            const uint32_t mine = (hi - lo + p.tile_rows - 1) / p.tile_rows;
+            uint32_t upto = mine;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= (uint32_t)o) upto += y;
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= (uint32_t)o) upto += y;
+            }
+            if (e < experts) { strips_before[e] = before + upto - mine; first_row[e] = lo; row_count[e] = hi - lo; }
+            before += __shfl_sync(0xffffffffu, upto, 31);
         }
-        const uint32_t found = __ballot_sync(0xffffffffu, slot < before + upto);
-        if (found) {
-            const int at = __ffs(found) - 1;
-            const uint32_t nt = __shfl_sync(0xffffffffu, tiles, at), all = __shfl_sync(0xffffffffu, rows, at);
-            const uint32_t first = before + __shfl_sync(0xffffffffu, upto, at) - nt, i = slot - first;
-            const uint32_t height = ((all + nt - 1) / nt + unit - 1) / unit * unit;
-            x.expert = e0 + at;
-            x.row0 = __shfl_sync(0xffffffffu, lo, at) + i * height;
-            x.rows = i * height < all ? min(height, all - i * height) : 0u;
-            x.tiles_before = first;
-            return true;
-        }
-        before += __shfl_sync(0xffffffffu, upto, 31);
+        if (lane == 0) strips_before[experts] = before;
     }
-    return false;
-}
+    // Tile t of strips() * n_blocks: inside an expert the channel blocks advance, strip fastest, so that its weights come from HBM once.
+    // Heights are rounded up to a multiple of `unit`.
+    __device__ __forceinline__ void tile(const ExpertParams& p, uint32_t t, uint32_t unit, ExpertStrip& s) const {
+        const uint32_t q = t / p.n_blocks;
+        uint32_t lo = 0, hi = experts;   // the expert with strips_before[e] <= q < strips_before[e + 1]
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (strips_before[mid] <= q) lo = mid; else hi = mid;
+        }
+        const uint32_t first = strips_before[lo], of = strips_before[lo + 1] - first, r = t - first * p.n_blocks, i = r % of, all = row_count[lo];
+        s.expert = lo;
+        s.block = r / of;
+        s.height = ((all + of - 1) / of + unit - 1) / unit * unit;
+        s.row0 = first_row[lo] + i * s.height;
+        s.rows = i * s.height < all ? min(s.height, all - i * s.height) : 0u;
+    }
+};
 
 // Row of A behind row r of C; a value outside [0, a_rows): none, reads as zeros.
 __device__ __forceinline__ uint32_t source_row(const ExpertParams& p, uint32_t r) {

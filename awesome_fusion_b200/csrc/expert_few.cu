@@ -3,287 +3,354 @@
 //
 //   D[n, r] = sum_k W[e][n,k] * A[row(r),k],   16 channels x 8 rows per mma.sync.m16n8k16, the channels as the row operand
 //
-// A cluster of S CTAs (1 to 8) owns 128 channels of one expert and up to 8 * MT of its rows; each CTA has a stretch of K, each of its eight
-// warps 16 channels.  A lane reads the 16 bytes of its two channels (16 or 32 consecutive k) straight into registers, four chunks ahead,
-// and unpacks them there (dequant.cuh).  The rows of A are staged in shared memory once per pass, in the order of k that the
-// unpack yields: a dot product does not care.  Group scales multiply the fp32 sum of a chunk, which lies in one group (HALF: in two, int4 in
-// groups of 64; a lane's 16 bytes are then 8 of each).  The CTAs of a cluster add their fp32 sums through distributed shared memory in the
-// order of k: no workspace, no counter, the same bits in every run.
-#include <cooperative_groups.h>
+// One CTA per SM walks tiles of 128 channels of one expert x up to 8 * MT of its rows; the weights of the next tiles are on their way while
+// one is worked on, in a ring of kStages stages of 128 bytes of k (256 int4, 128 int8):
+//
+//   warps 0-15   32 channels each; four warps share a stage, the four fours take every fourth stage.  A lane reads 16 bytes of four channels and
+//                32 bytes of a row of A per 16 (int8) or 32 (int4) k of its own, unpacks the weights in registers (dequant.cuh) and feeds mma.sync: the
+//                four lanes of a quad hold different k.  At the end of a tile the fours' sums meet in shared memory.
+//   warps 16-19  the rows of A, 16-byte copies that report to the stage's barrier by themselves; warp 16 also the raw weights by TMA, two boxes of 128
+//                channels x 64 bytes: rows of 64 bytes are read without bank conflicts as they lie
+//
+// Group scales multiply the fp32 sum of 64 bytes of k, which lie in one group (HALF: in two, int4 in groups of 64; a lane's 16 bytes are then 8 of each).
+// No workspace, no counter, the same bits in every run.
 #include "dequant.cuh"
 #include "decode_common.cuh"
 #include "expert_common.cuh"
+#include "stream_common.cuh"
 
 namespace afb {
 namespace {
 
-constexpr int kAhead = 4;             // chunks of weights in registers
-constexpr uint32_t kFewChannels = 128;
-constexpr uint32_t kSumPitch = 132;   // floats per row of the CTA's sums: 16-byte rows, banks shifted by 4
+constexpr int kFewWarps = 16, kLoadWarps = 4, kFewThreads = 32 * (kFewWarps + kLoadWarps);   // 640: launched with 96 registers a thread
+constexpr uint32_t kRegsWork = 112, kRegsLoad = 32;
+static_assert(32 * kFewWarps * kRegsWork + 32 * kLoadWarps * kRegsLoad <= 96 * kFewThreads, "shares of the registers");
+constexpr uint32_t kWays = 4, kStages = 8;     // kStages: a multiple of kWays, so that a warp meets every phase of the stages that it meets
+constexpr uint32_t kHalfBytes = kCh * 64;      // a box of weights
+constexpr uint32_t kSumPitch = kCh + 4;        // floats per row of a way's sums
+constexpr int kOffBars = 0, kOffStage = 256;   // two barriers per stage, the abort flag
+static_assert(kLoadWarps % 2 == 0 && kStages % kWays == 0 && 16 * kStages + 8 <= kOffStage, "ring");
 
-template <bool HALF> struct Chunk {
-    uint4 wa, wb;
-    float sa[HALF ? 2 : 1], sb[HALF ? 2 : 1];
-    uint32_t za[HALF ? 2 : 1], zb[HALF ? 2 : 1];   // the unpack's addends, where there are zero-points
+struct FewParams {
+    ExpertParams x;
+    uint32_t stages_per_tile;   // along K
+    uint32_t off_sums, off_table;
+    int32_t* status;
 };
 
-__device__ __forceinline__ uint4 ldg_weights(const uint8_t* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
+__device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-__device__ __forceinline__ uint2 ldg_weights8(const uint8_t* p) {
+// `bytes` (0 or 16) from src, zeros behind them.
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// Arrives on `bar` when this thread's copies so far are complete.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
     uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
     return v;
 }
+// Place of 16-byte piece `pc` of a row of A: the eight lanes that read at once hold two rows and, of int4, pieces 4 apart.
+__device__ __forceinline__ uint32_t act_place(uint32_t row, uint32_t pc) { return pc ^ (((pc >> 3) & 1u) << 1) ^ (row & 1u); }
 
 template <int BITS, int MT, bool GROUPED, bool HALF>
-__global__ void __launch_bounds__(kThreads, MT == 4 ? 1 : 2)
-expert_few_kernel(const ExpertParams p, const uint32_t split, const uint32_t pass_chunks, const uint32_t row_bytes) {
-    constexpr uint32_t CH = BITS == 8 ? 64 : 128, LK = CH / 4, AV = LK / 8;   // k per chunk; k per lane; 16-byte pieces of A per lane
-    extern __shared__ __align__(16) uint8_t smem[];
-    const uint32_t s_act = (uint32_t)__cvta_generic_to_shared(smem);
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tig = lane & 3;
-    const uint32_t rank = blockIdx.x % split, unit = blockIdx.x / split;   // the CTAs of a cluster are consecutive
-    ExpertTile t;
-    if (!find_tile(p, unit / p.n_blocks, 1, lane, t)) return;              // the whole cluster alike
-    const uint32_t n0 = unit % p.n_blocks * kFewChannels;
+__global__ void __launch_bounds__(kFewThreads, 1)
+expert_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const FewParams p) {
+    constexpr uint32_t CH = BITS == 8 ? 64 : 128, LK = CH / 4, AV = LK / 8;   // k per 64 bytes; of them per lane; 16-byte pieces of A per lane
+    constexpr uint32_t kRowBytes = 2 * CH * 2;                                // of A per stage
+    constexpr uint32_t kStageAct = 8 * MT * kRowBytes, kStageAll = 2 * kHalfBytes + kStageAct;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const uint32_t base = ptx::smem_u32(smem);
+    const ExpertParams& x = p.x;
+    auto full = [&](uint32_t s) { return base + kOffBars + 8u * s; };
+    auto empty = [&](uint32_t s) { return base + kOffBars + 8u * (kStages + s); };
+    volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + 16 * kStages);
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const ExpertTable table(smem + p.off_table, x.experts);
 
-    const uint32_t row_a = n0 + warp * 16 + g, row_b = row_a + 8;
-    const bool ok_a = row_a < p.n, ok_b = row_b < p.n;
-    const size_t chan_a = (size_t)t.expert * p.n + (ok_a ? row_a : 0), chan_b = (size_t)t.expert * p.n + (ok_b ? row_b : 0);
-    const uint32_t chunks = p.k / CH, c0 = (uint32_t)((uint64_t)chunks * rank / split), nch = (uint32_t)((uint64_t)chunks * (rank + 1) / split) - c0;
-    const uint8_t* pa = p.b + chan_a * p.ldb_bytes + (size_t)c0 * 64 + tig * (HALF ? 8 : 16);
-    const uint8_t* pb = p.b + chan_b * p.ldb_bytes + (size_t)c0 * 64 + tig * (HALF ? 8 : 16);
-    const uint32_t groups_per_row = GROUPED ? p.k >> p.group_shift : 0;
-    const uint32_t flip = BITS == 8 ? flip8(p.enc) : flip4(p.enc);
-    uint32_t add_a = unpack_add(BITS, 0), add_b = add_a;
-    const bool has_zero = p.zero != nullptr;
-    auto zero_add = [&](size_t i) { return unpack_add(BITS, BITS == 8 ? decode_zero8(p.zero[i], p.enc) : decode_zero4(p.zero[i], p.enc)); };
-    if (!GROUPED && has_zero) { add_a = zero_add(chan_a); add_b = zero_add(chan_b); }
-
-    auto load = [&](Chunk<HALF>& q, uint32_t c) {   // chunk c of this CTA's stretch
-        if (HALF) {
-            const uint2 a0 = ldg_weights8(pa + (size_t)c * 64), a1 = ldg_weights8(pa + (size_t)c * 64 + 32);
-            const uint2 b0 = ldg_weights8(pb + (size_t)c * 64), b1 = ldg_weights8(pb + (size_t)c * 64 + 32);
-            q.wa = make_uint4(a0.x, a0.y, a1.x, a1.y); q.wb = make_uint4(b0.x, b0.y, b1.x, b1.y);
-        } else {
-            q.wa = ldg_weights(pa + (size_t)c * 64); q.wb = ldg_weights(pb + (size_t)c * 64);
+    if (warp == kFewWarps) {
+        if (lane == 0) {
+            for (uint32_t s = 0; s < kStages; ++s) { ptx::mbar_init(full(s), 1 + 32 * kLoadWarps); ptx::mbar_init(empty(s), kWays); }
+            *abort_flag = 0;
+            ptx::fence_mbar_init();
+            ptx::prefetch_tmap(&tmap_w);
         }
-        if (GROUPED) {
-#pragma unroll
-            for (int h = 0; h < (HALF ? 2 : 1); ++h) {
-                const uint32_t grp = ((c0 + c) * CH + h * (CH / 2)) >> p.group_shift;
-                const size_t ia = chan_a * groups_per_row + grp, ib = chan_b * groups_per_row + grp;
-                q.sa[h] = load_scale(p.scale, ia, p.scale_dtype); q.sb[h] = load_scale(p.scale, ib, p.scale_dtype);
-                if (has_zero) { q.za[h] = zero_add(ia); q.zb[h] = zero_add(ib); }
-            }
-        }
-    };
-    Chunk<HALF> q[kAhead];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) if ((uint32_t)u < nch) load(q[u], u);
-
-    // B operand: lane (g, tig) reads row g's k of lane tig.  Rows behind the last one read row 0; their columns of D are never stored.
-    uint32_t act_base[MT], act_off[AV];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) act_base[mt] = s_act + (mt * 8 + g < t.rows ? mt * 8 + g : 0) * row_bytes;
-    // 16-byte pieces of a chunk; int4 with whole groups: bit 3 of the piece flips bit 1, else lanes 0 and 2 of a quad share a bank
-    constexpr bool kSwizzle = BITS == 4 && !HALF;
-#pragma unroll
-    for (uint32_t v = 0; v < AV; ++v) {
-        const uint32_t piece = HALF ? (v / 2) * 8 + tig * 2 + (v & 1) : tig * AV + v;
-        act_off[v] = (kSwizzle ? swz_piece(piece) : piece) * 16;
+        __syncwarp();
+    } else if (warp == 0) {
+        table.build(x, lane);
     }
-    float acc[MT][4];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[mt][e] = 0.f;
-
-    auto consume = [&](const Chunk<HALF>& q, uint32_t coff) {   // coff: byte offset of the chunk in a staged row
-        const uint32_t wa[4] = {q.wa.x, q.wa.y, q.wa.z, q.wa.w}, wb[4] = {q.wb.x, q.wb.y, q.wb.z, q.wb.w};
-        float part[MT][4];
-        if (GROUPED) {
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) part[mt][e] = 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int h = HALF ? j / 2 : 0;
-            const uint32_t aa = GROUPED && has_zero ? q.za[h] : add_a, ab = GROUPED && has_zero ? q.zb[h] : add_b;
-            uint32_t fa[4], fb[4];
-            if (BITS == 8) {
-                s8x4_to_bf16(wa[j], flip, kSel8Strided02, kSel8Strided13, kMulByte, aa, fa[0], fa[1]);
-                s8x4_to_bf16(wb[j], flip, kSel8Strided02, kSel8Strided13, kMulByte, ab, fb[0], fb[1]);
-            } else {
-                s4x8_to_bf16_strided(wa[j], flip, aa, fa);
-                s4x8_to_bf16_strided(wb[j], flip, ab, fb);
-            }
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                if (mt * 8 >= (int)t.rows && mt > 0) break;
-                float (&d)[4] = GROUPED ? part[mt] : acc[mt];
-                if (BITS == 8) {
-                    const uint4 x = lds128(act_base[mt] + coff + act_off[j / 2]);   // two words' worth: the compiler reads it once
-                    if (j % 2 == 0) mma_bf16(d, fa[0], fb[0], fa[1], fb[1], x.x, x.y);
-                    else            mma_bf16(d, fa[0], fb[0], fa[1], fb[1], x.z, x.w);
-                } else {
-                    const uint4 x = lds128(act_base[mt] + coff + act_off[j]);
-                    mma_bf16(d, fa[0], fb[0], fa[1], fb[1], x.x, x.y);
-                    mma_bf16(d, fa[2], fb[2], fa[3], fb[3], x.z, x.w);
-                }
-            }
-            if (GROUPED && (j == 3 || (HALF && j == 1))) {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    acc[mt][0] = fmaf(q.sa[h], part[mt][0], acc[mt][0]); acc[mt][1] = fmaf(q.sa[h], part[mt][1], acc[mt][1]);
-                    acc[mt][2] = fmaf(q.sb[h], part[mt][2], acc[mt][2]); acc[mt][3] = fmaf(q.sb[h], part[mt][3], acc[mt][3]);
-                    if (HALF) part[mt][0] = part[mt][1] = part[mt][2] = part[mt][3] = 0.f;
-                }
-            }
-        }
-    };
-
-    // threads per row of A when staging: all 256 for one row, 32 for eight and more
-    const uint32_t per_row = t.rows >= 5 ? 32u : t.rows >= 3 ? 64u : t.rows == 2 ? 128u : 256u;
-    for (uint32_t p0 = 0; p0 < nch; p0 += pass_chunks) {
-        const uint32_t in_pass = min(pass_chunks, nch - p0);
-        if (p0) __syncthreads();   // the previous pass has been consumed by every warp
-        const uint32_t pieces = in_pass * (CH / 8);
-        for (uint32_t r = tid / per_row; r < t.rows; r += kThreads / per_row) {
-            const uint32_t src_row = source_row(p, t.row0 + r);
-            const uint16_t* src = p.a + (size_t)src_row * p.lda + (size_t)(c0 + p0) * CH;
-            const bool there = src_row < p.a_rows;
-#pragma unroll 4
-            for (uint32_t pc = tid % per_row; pc < pieces; pc += per_row) {
-                const uint4 v = there ? ldg_act(src + (size_t)pc * 8) : make_uint4(0u, 0u, 0u, 0u);
-                uint4 o;
-                if (p.packed) {           // pre-packed weights unpack to consecutive k
-                    o = v;
-                } else if (BITS == 8) {   // {k0,k2},{k1,k3},{k4,k6},{k5,k7}
-                    o.x = prmt(v.x, v.y, 0x5410u); o.y = prmt(v.x, v.y, 0x7632u);
-                    o.z = prmt(v.z, v.w, 0x5410u); o.w = prmt(v.z, v.w, 0x7632u);
-                } else {                  // {k0,k4},{k1,k5},{k2,k6},{k3,k7}
-                    o.x = prmt(v.x, v.z, 0x5410u); o.y = prmt(v.x, v.z, 0x7632u);
-                    o.z = prmt(v.y, v.w, 0x5410u); o.w = prmt(v.y, v.w, 0x7632u);
-                }
-                *reinterpret_cast<uint4*>(smem + r * row_bytes + (kSwizzle ? swz_piece(pc) : pc) * 16) = o;
-            }
-        }
-        __syncthreads();
-        for (uint32_t i = 0; i < in_pass; i += kAhead) {   // pass_chunks is a multiple of kAhead: chunk p0 + i is in q[0]
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                if (i + u >= in_pass) break;
-                consume(q[u], (i + u) * (CH * 2));
-                if (p0 + i + u + kAhead < nch) load(q[u], p0 + i + u + kAhead);
-            }
-        }
-    }
-
-    // ---- the sums meet in shared memory: [row][channel] of every CTA, added up in the order of the ranks
     __syncthreads();
-    float* sums = reinterpret_cast<float*>(smem);
+    auto give_up = [&](int where, uint32_t a, uint32_t b) {
+        if (!*abort_flag) { report_timeout(p.status, where, (int)a, (int)b); *abort_flag = 1; }
+    };
+    const uint32_t tiles = table.strips() * x.n_blocks, ns = p.stages_per_tile;
+    ExpertStrip t;
+
+    if (warp >= kFewWarps) {
+        ptx::regs_down<kRegsLoad>();
+        // ======================= weights and rows of A =======================
+        constexpr uint32_t kPieces = kRowBytes / 16, kRowsAtOnce = 32 / kPieces, kTurn = kLoadWarps * kRowsAtOnce;   // of one warp's copy; of all warps'
+        const uint32_t r0 = (warp - kFewWarps) * kRowsAtOnce + lane / kPieces, piece = lane % kPieces;
+        // the halves of a stage one after the other: the pieces of 64 bytes of weights, for every row
+        const uint32_t half = piece / (kPieces / 2), pc = piece % (kPieces / 2);
+        const uint32_t dst = 2 * kHalfBytes + half * (kStageAct / 2) + r0 * (kRowBytes / 2) + act_place(r0, pc) * 16u;   // kTurn rows on: the same place
+        Ring r{0, 0};
+        uint32_t issued = 0, parity = 0;
+        bool ok = true;
+        for (uint32_t i = blockIdx.x; ok && i < tiles; i += gridDim.x) {
+            table.tile(x, i, 1, t);
+            const int y = (int)(t.expert * x.n + t.block * kCh);
+            const uint16_t* src[8 * MT / kTurn];   // of this lane's piece of the next stage
+            uint32_t size[8 * MT / kTurn];         // bytes that there are of it; the rest is zeros
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+            for (uint32_t j = 0; j < 8 * MT / kTurn; ++j) {
+                const uint32_t row = r0 + j * kTurn < t.rows ? source_row(x, t.row0 + r0 + j * kTurn) : 0xffffffffu;
+                size[j] = row < x.a_rows ? 16u : 0u;
+                src[j] = x.a + (size[j] ? (size_t)row * x.lda : 0) + piece * 8u;
+            }
+            for (uint32_t kb = 0; kb < ns; ++kb) {
+                if (!warp_wait(empty(r.i), r.phase ^ 1u, abort_flag)) { give_up(71, i, kb); ok = false; break; }
+                const uint32_t stage = base + kOffStage + r.i * kStageAll;
+                if (warp == kFewWarps && ptx::elect_one()) {
+                    ptx::mbar_arrive_expect_tx(full(r.i), 2 * kHalfBytes);
+                    ptx::tma_load_2d(stage, &tmap_w, (int)(kb * 128u), y, full(r.i));
+                    ptx::tma_load_2d(stage + kHalfBytes, &tmap_w, (int)(kb * 128u + 64u), y, full(r.i));
+                }
+                __syncwarp();
+                const bool inside = kb * (2 * CH) + piece * 8u < x.k;   // the last stage may have but one half
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (mt * 8 + 2 * tig + (e & 1) < t.rows)
-                sums[(mt * 8 + 2 * tig + (e & 1)) * kSumPitch + warp * 16 + g + (e >> 1) * 8] = acc[mt][e];
-    namespace cg = cooperative_groups;
-    if (split > 1) cg::this_cluster().sync(); else __syncthreads();
-    const uint32_t vecs = t.rows * (kFewChannels / 4);
-    for (uint32_t v = rank * kThreads + tid; v < vecs; v += split * kThreads) {
-        const uint32_t r = v / (kFewChannels / 4), ch = v % (kFewChannels / 4) * 4, nn = n0 + ch;
-        if (nn >= p.n) continue;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (split == 1) {
-            x = *reinterpret_cast<const float4*>(sums + r * kSumPitch + ch);
-        } else {
-            for (uint32_t c = 0; c < split; ++c) {
-                const float4 y = *reinterpret_cast<const float4*>(cg::this_cluster().map_shared_rank(sums, c) + r * kSumPitch + ch);
-                x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+                for (uint32_t j = 0; j < 8 * MT / kTurn; ++j) {
+                    if (r0 + j * kTurn >= t.rows) break;   // the columns of D of the rows behind the last one are never stored
+                    cp_async16_or_zero(stage + dst + j * (kTurn * kRowBytes / 2), inside ? src[j] : x.a, inside ? size[j] : 0u);
+                    src[j] += 2 * CH;
+                }
+                cp_async_arrive(full(r.i));
+                issued |= 1u << r.i; parity = (parity & ~(1u << r.i)) | (r.phase << r.i);
+                r.step(1, kStages);
             }
         }
-        float f[4] = {x.x, x.y, x.z, x.w};
+        cp_async_wait<0>();   // never leave with a copy still writing this CTA's shared memory
+        for (uint32_t s = 0; s < kStages; ++s)
+            if (issued & (1u << s)) ptx::mbar_wait(full(s), (parity >> s) & 1u);
+    } else {
+        // ======================= 32 channels x one of the ways =======================
+        ptx::regs_up<kRegsWork>();
+        const uint32_t cg = warp & 3u, way = warp >> 2, g = lane >> 2, tig = lane & 3;
+        const uint32_t flip = BITS == 8 ? flip8(x.enc) : flip4(x.enc);
+        const uint32_t sel0 = x.packed ? kSel8Strided02 : kSel8Natural01, sel1 = x.packed ? kSel8Strided13 : kSel8Natural23;
+        const Nibbles nib = nibbles(x.packed != 0);
+        const bool has_zero = x.zero != nullptr, half_scale = x.scale_dtype == AFB_SCALE_BF16;
+        const uint32_t groups_per_row = GROUPED ? x.k >> x.group_shift : 0;
+        constexpr int kGroupsPer = GROUPED ? (HALF ? 4 : 2) : 1;   // scale groups of a stage, at most
+        uint32_t act_off[AV];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (GROUPED) f[e] *= kUnpackInverse;
-            else f[e] = nn + e < p.n ? unscaled(f[e], load_scale(p.scale, (size_t)t.expert * p.n + nn + e, p.scale_dtype)) : 0.f;
-        }
-        if (p.gated) {
-            uint16_t* dst = p.c + (size_t)(t.row0 + r) * p.ldc + nn / 2;
+        for (uint32_t v = 0; v < AV; ++v) act_off[v] = act_place(g, HALF ? (v / 2) * 8 + tig * 2 + (v & 1) : tig * AV + v) * 16u + g * (kRowBytes / 2);   // eight rows on: the same place
+        const uint32_t raw_off = (cg * 32 + g) * 64 + tig * (HALF ? 8 : 16);
+        float* sums = reinterpret_cast<float*>(smem + p.off_sums);
+        uint32_t before = 0;   // stages of the tiles walked so far
+        bool ok = true;
+        for (uint32_t i = blockIdx.x; i < tiles; i += gridDim.x) {
+            table.tile(x, i, 1, t);
+            const uint32_t n0 = t.block * kCh;
+            uint32_t chan[4];      // rows of B of this lane's channels: 8 apart
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                if (nn + 2 * e < p.n) dst[e] = __bfloat16_as_ushort(__float2bfloat16_rn((p.silu ? silu(f[2 * e]) : f[2 * e]) * f[2 * e + 1]));
-        } else {
-            uint16_t* dst = p.c + (size_t)(t.row0 + r) * p.ldc + nn;
+            for (int j = 0; j < 4; ++j) chan[j] = t.expert * x.n + min(n0 + cg * 32 + j * 8 + g, x.n - 1);
+            auto zero_add = [&](size_t at) { return unpack_add(BITS, BITS == 8 ? decode_zero8(x.zero[at], x.enc) : decode_zero4(x.zero[at], x.enc)); };
+            uint32_t add[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (nn + e < p.n) dst[e] = __bfloat16_as_ushort(__float2bfloat16_rn(p.silu ? silu(f[e]) : f[e]));
+            for (int j = 0; j < 4; ++j) add[j] = !GROUPED && has_zero ? zero_add(chan[j]) : unpack_add(BITS, 0);
+            // scales and zero-points of this warp's next stage, as they are stored: fetched when it is done with the one before, converted (which
+            // waits for them) when they are used
+            uint32_t sc[kGroupsPer][4], zp[kGroupsPer][4];
+            auto load_scales = [&](uint32_t kb) {
+                if constexpr (!GROUPED) return;
+                if (kb >= ns) return;
+#pragma unroll
+                for (int q = 0; q < kGroupsPer; ++q) {
+                    const uint32_t k = kb * (2 * CH) + q * (2 * CH / kGroupsPer);
+                    if (k >= x.k) break;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const size_t at = (size_t)chan[j] * groups_per_row + (k >> x.group_shift);
+                        sc[q][j] = half_scale ? reinterpret_cast<const uint16_t*>(x.scale)[at] : reinterpret_cast<const uint32_t*>(x.scale)[at];
+                        if (has_zero) zp[q][j] = x.zero[at];
+                    }
+                }
+            };
+            auto scale_of = [&](uint32_t raw) { return __uint_as_float(half_scale ? raw << 16 : raw); };
+            float acc[2][MT][4];
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int nt = 0; nt < MT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[m][nt][e] = 0.f;
+            uint32_t kb = (way - before) & (kWays - 1);
+            Ring r;
+            r.set(before + kb, kStages);
+            load_scales(kb);
+            for (; kb < ns; kb += kWays) {
+                ok = ok && warp_wait(full(r.i), r.phase, abort_flag);
+                if (!ok) { give_up(73, i, kb); break; }
+                const uint32_t stage = base + kOffStage + r.i * kStageAll;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {   // 64 bytes of k
+                    if (c == 1 && kb * (2 * CH) + CH >= x.k) break;
+                    const uint32_t raw = stage + c * kHalfBytes + raw_off, act = stage + 2 * kHalfBytes + c * (kStageAct / 2);
+                    uint32_t w[4][4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (HALF) {
+                            const uint2 lo = lds64(raw + j * 512), hi = lds64(raw + j * 512 + 32);
+                            w[j][0] = lo.x; w[j][1] = lo.y; w[j][2] = hi.x; w[j][3] = hi.y;
+                        } else {
+                            const uint4 v = lds128(raw + j * 512);
+                            w[j][0] = v.x; w[j][1] = v.y; w[j][2] = v.z; w[j][3] = v.w;
+                        }
+                    }
+                    float part[2][MT][4];
+                    uint4 b[MT];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {   // words of the 16 bytes
+                        const int grp = !GROUPED ? 0 : HALF ? 2 * c + q / 2 : c;
+                        if (GROUPED && has_zero && (q == 0 || (HALF && q == 2))) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) add[j] = unpack_add(BITS, BITS == 8 ? decode_zero8(zp[grp][j], x.enc) : decode_zero4(zp[grp][j], x.enc));
+                        }
+                        if (BITS == 4 || q % 2 == 0) {
+#pragma unroll
+                            for (int nt = 0; nt < MT; ++nt) b[nt] = lds128(act + act_off[BITS == 4 ? q : q / 2] + nt * (8 * kRowBytes / 2));
+                        }
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            uint32_t fa[4], fb[4];
+                            const uint32_t aa = add[2 * m], ab = add[2 * m + 1];
+                            if (BITS == 8) {
+                                s8x4_to_bf16(w[2 * m][q], flip, sel0, sel1, kMulByte, aa, fa[0], fa[1]);
+                                s8x4_to_bf16(w[2 * m + 1][q], flip, sel0, sel1, kMulByte, ab, fb[0], fb[1]);
+                            } else {
+                                s4x8_to_bf16(w[2 * m][q], flip, nib, nib.mul[0], nib.mul[1], aa, fa);
+                                s4x8_to_bf16(w[2 * m + 1][q], flip, nib, nib.mul[0], nib.mul[1], ab, fb);
+                            }
+                            const bool first = GROUPED && (q == 0 || (HALF && q == 2)), last = GROUPED && (q == 3 || (HALF && q == 1));
+#pragma unroll
+                            for (int nt = 0; nt < MT; ++nt) {
+                                if (BITS == 8) {
+                                    const uint32_t b0 = q % 2 == 0 ? b[nt].x : b[nt].z, b1 = q % 2 == 0 ? b[nt].y : b[nt].w;
+                                    if (!GROUPED) mma_bf16(acc[m][nt], fa[0], fb[0], fa[1], fb[1], b0, b1);
+                                    else if (first) mma_bf16_first(part[m][nt], fa[0], fb[0], fa[1], fb[1], b0, b1);
+                                    else mma_bf16(part[m][nt], fa[0], fb[0], fa[1], fb[1], b0, b1);
+                                } else {
+                                    if (!GROUPED) mma_bf16(acc[m][nt], fa[0], fb[0], fa[1], fb[1], b[nt].x, b[nt].y);
+                                    else if (first) mma_bf16_first(part[m][nt], fa[0], fb[0], fa[1], fb[1], b[nt].x, b[nt].y);
+                                    else mma_bf16(part[m][nt], fa[0], fb[0], fa[1], fb[1], b[nt].x, b[nt].y);
+                                    mma_bf16(GROUPED ? part[m][nt] : acc[m][nt], fa[2], fb[2], fa[3], fb[3], b[nt].z, b[nt].w);
+                                }
+                                if (last) {
+                                    const float sa = scale_of(sc[grp][2 * m]), sb = scale_of(sc[grp][2 * m + 1]);
+                                    acc[m][nt][0] = fmaf(sa, part[m][nt][0], acc[m][nt][0]); acc[m][nt][1] = fmaf(sa, part[m][nt][1], acc[m][nt][1]);
+                                    acc[m][nt][2] = fmaf(sb, part[m][nt][2], acc[m][nt][2]); acc[m][nt][3] = fmaf(sb, part[m][nt][3], acc[m][nt][3]);
+                                }
+                            }
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(empty(r.i));
+                load_scales(kb + kWays);
+                r.step(kWays, kStages);
+            }
+            before += ns;
+            // ---- the ways' sums meet: [way][row][channel], added in the order of the ways.  (Also after an abort: the barriers count all warps.)
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int nt = 0; nt < MT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        sums[(way * (8 * MT) + nt * 8 + 2 * tig + (e & 1)) * kSumPitch + cg * 32 + m * 16 + (e >> 1) * 8 + g] = acc[m][nt][e];
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kFewWarps) : "memory");
+            const uint32_t row = tid / (kCh / 4), ch = tid % (kCh / 4) * 4, nn = n0 + ch;
+            if (row < t.rows && nn < x.n) {
+                float f[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (uint32_t wy = 0; wy < kWays; ++wy) {
+                    const float4 y = *reinterpret_cast<const float4*>(sums + (wy * (8 * MT) + row) * kSumPitch + ch);
+                    f[0] += y.x; f[1] += y.y; f[2] += y.z; f[3] += y.w;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (GROUPED) f[e] *= kUnpackInverse;
+                    else f[e] = nn + e < x.n ? unscaled(f[e], load_scale(x.scale, (size_t)t.expert * x.n + nn + e, x.scale_dtype)) : 0.f;
+                }
+                if (x.gated) {
+                    uint16_t* dst = x.c + (size_t)(t.row0 + row) * x.ldc + nn / 2;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        if (nn + 2 * e < x.n) dst[e] = __bfloat16_as_ushort(__float2bfloat16_rn((x.silu ? silu(f[2 * e]) : f[2 * e]) * f[2 * e + 1]));
+                } else {
+                    uint16_t* dst = x.c + (size_t)(t.row0 + row) * x.ldc + nn;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (nn + e < x.n) dst[e] = __bfloat16_as_ushort(__float2bfloat16_rn(x.silu ? silu(f[e]) : f[e]));
+                }
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kFewWarps) : "memory");
         }
     }
-    if (split > 1) cg::this_cluster().sync();   // no CTA leaves while another reads its sums
 }
 
 template <int BITS, int MT, bool GROUPED, bool HALF>
-int launch_cfg(const ExpertParams& p, uint32_t split, DeviceCtx* ctx, cudaStream_t s) {
+int launch_cfg(const CUtensorMap& tw, const FewParams& q, DeviceCtx* ctx, cudaStream_t s) {
     auto kern = expert_few_kernel<BITS, MT, GROUPED, HALF>;
-    constexpr uint32_t CH = BITS == 8 ? 64 : 128;
-    // rows of A in shared memory: 32 KiB (48 from 16 rows on) for two CTAs per SM and more
-    const uint32_t most = MT == 4 ? 96 * 1024 : MT == 2 ? 64 * 1024 : 32 * 1024;
-    const uint32_t chunks = (p.k / CH + split - 1) / split;
-    uint32_t pass = (most / p.tile_rows - 16) / (CH * 2) / kAhead * kAhead;
-    const uint32_t whole = (chunks + kAhead - 1) / kAhead * kAhead;
-    if (pass > whole) pass = whole;
-    const uint32_t row_bytes = pass * CH * 2 + 16;   // + 16: consecutive rows lie in different banks
-    uint32_t bytes = p.tile_rows * row_bytes;
-    if (bytes < p.tile_rows * kSumPitch * 4) bytes = p.tile_rows * kSumPitch * 4;
+    FewParams p = q;
+    p.off_sums = kOffStage + kStages * (2 * kHalfBytes + 8 * MT * (BITS == 8 ? 256 : 512));
+    p.off_table = p.off_sums + kWays * 8 * MT * kSumPitch * sizeof(float);
+    const uint32_t bytes = p.off_table + ExpertTable::bytes(p.x.experts);
+    if (bytes > 232448) return AFB_ERR_UNSUPPORTED;   // the caller has seen to it
     static DeviceOnce attr_set;
     if (!attr_set.done(ctx->device)) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024 + 1024);
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
         if (e != cudaSuccess) return cuda_fail(e);
         attr_set.mark(ctx->device);
     }
-    const uint64_t grid = expert_tiles(p.m, p.experts, p.tile_rows) * p.n_blocks * split;
-    if (grid >> 31) return AFB_ERR_TOO_LARGE;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((uint32_t)grid); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = bytes; cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr; cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, split, pass, row_bytes);
+    const uint64_t tiles = expert_tiles(p.x.m, p.x.experts, p.x.tile_rows) * p.x.n_blocks;
+    if (tiles >> 31) return AFB_ERR_TOO_LARGE;
+    const uint32_t grid = tiles < (uint64_t)ctx->sm_count ? (uint32_t)tiles : (uint32_t)ctx->sm_count;
+    kern<<<grid, kFewThreads, bytes, s>>>(tw, p);
     count_launch();
+    const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? AFB_OK : cuda_fail(e);
 }
 
 template <int MT>
-int launch_rows(const ExpertParams& p, uint32_t bits, uint32_t group, uint32_t split, DeviceCtx* ctx, cudaStream_t s) {
-    if (bits == 8) return group ? launch_cfg<8, MT, true, false>(p, split, ctx, s) : launch_cfg<8, MT, false, false>(p, split, ctx, s);
-    if (group == 64) return launch_cfg<4, MT, true, true>(p, split, ctx, s);
-    return group ? launch_cfg<4, MT, true, false>(p, split, ctx, s) : launch_cfg<4, MT, false, false>(p, split, ctx, s);
+int launch_rows(const CUtensorMap& tw, const FewParams& p, uint32_t bits, uint32_t group, DeviceCtx* ctx, cudaStream_t s) {
+    if (bits == 8) return group ? launch_cfg<8, MT, true, false>(tw, p, ctx, s) : launch_cfg<8, MT, false, false>(tw, p, ctx, s);
+    if (group == 64) return launch_cfg<4, MT, true, true>(tw, p, ctx, s);
+    return group ? launch_cfg<4, MT, true, false>(tw, p, ctx, s) : launch_cfg<4, MT, false, false>(tw, p, ctx, s);
 }
 
 }  // namespace
 
 int launch_expert_few(const ExpertParams& q, uint32_t bits, uint32_t group, DeviceCtx* ctx, cudaStream_t s) {
-    ExpertParams p = q;
-    p.n_blocks = (p.n + kFewChannels - 1) / kFewChannels;
-    const uint32_t mean = (p.m + p.experts - 1) / p.experts;   // rows per expert
-    const uint32_t mt = mean <= 2 ? 1 : mean <= 12 ? 2 : 4;
-    p.tile_rows = 8 * mt;
-    // stretches of K: enough CTAs for two waves of two per SM, at least four chunks each
-    const uint32_t chunks = p.k / (bits == 8 ? 64 : 128);
-    const uint64_t ctas = expert_tiles(p.m, p.experts, p.tile_rows) * p.n_blocks;
-    uint32_t split = 1;
-    while (split < 8 && ctas * split < 4ull * ctx->sm_count && chunks >= split * 2 * kAhead) split *= 2;
-    return mt == 1 ? launch_rows<1>(p, bits, group, split, ctx, s) : mt == 2 ? launch_rows<2>(p, bits, group, split, ctx, s)
-                                                                             : launch_rows<4>(p, bits, group, split, ctx, s);
+    FewParams p{};
+    p.x = q;
+    p.x.n_blocks = (q.n + kCh - 1) / kCh;
+    p.stages_per_tile = (uint32_t)(((uint64_t)q.k * bits / 8 + 127) / 128);
+    p.status = ctx->status;
+    // tiles of 8 rows where few experts have more; of int4 also where the table of many experts leaves no room for the rows of 16
+    const bool small = (uint64_t)q.m <= 3ull * q.experts || (bits == 4 && q.experts > 128);
+    p.x.tile_rows = small ? 8 : 16;
+    CUtensorMap tw;
+    const int rc = tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.b, (uint64_t)q.k * bits / 8, (uint64_t)q.experts * q.n, q.ldb_bytes, 64, kCh, CU_TENSOR_MAP_SWIZZLE_NONE);
+    if (rc) return rc;
+    return small ? launch_rows<1>(tw, p, bits, group, ctx, s) : launch_rows<2>(tw, p, bits, group, ctx, s);
 }
 
 }  // namespace afb

@@ -8,8 +8,8 @@
 //   warp 0        TMA: raw weight blocks, 128 channels x 128 bytes, 128-byte swizzle
 //   warps 2, 3    rank 0: tcgen05.mma 256 x height x 16;  rank 1, warp 2: reports to rank 0 that its half of a step is complete
 //   warps 4-11    epilogue, two per lane quarter: accumulator -> registers -> (accumulator free) -> shared memory -> C
-//   warps 12-27   converters: four groups of four warps; group g takes every fourth step of k (KS = 128 or 64 wide)
-//   warps 28-31   the rows of A: 16-byte copies to shared memory, written in the 128-byte swizzle.  (A TMA gather of four rows takes 65 cycles of
+//   warps 12-19   converters: two groups of four warps; group g takes every second step of k (KS = 128 or 64 wide)
+//   warps 20-23   the rows of A: 16-byte copies to shared memory, written in the 128-byte swizzle.  (A TMA gather of four rows takes 65 cycles of
 //                 the issuing warp, which has to make every lane's row numbers uniform first: 4200 cycles per step of 256 rows.)
 //
 // Scales per channel: the sum over all of K stays in the accumulator, strips of up to 256 rows.
@@ -18,8 +18,7 @@
 // fp32 registers: strips of up to 128 rows (64 sums a thread).  A step is then 512 cycles of tensor work, less than one warp needs to issue it
 // (wait 80, eight MMAs 480, two commits 360): two warps issue, one per accumulator.
 //
-// A table in shared memory says where each expert's rows and strips begin; every role walks the same tiles from it: tile t = worker, worker +
-// workers, ...; inside an expert the channels advance, strip fastest, so that its weights are read from HBM once.
+// Every role walks the same tiles (ExpertTable): worker, worker + workers, ...
 #include "dequant.cuh"
 #include "expert_common.cuh"
 #include "stream_common.cuh"
@@ -27,10 +26,11 @@
 namespace afb {
 namespace {
 
-constexpr int kFirstEpi = 4, kEpiWarps = 8, kFirstConv = kFirstEpi + kEpiWarps, kFirstLoad = kFirstConv + 4 * kGroups, kLoadWarps = 4;
-constexpr int kManyThreads = 32 * (kFirstLoad + kLoadWarps);   // 1024: launched with 64 registers a thread
-constexpr uint32_t kRegsCtrl = 40, kRegsEpi = 104, kRegsConv = 56, kRegsLoad = 40;
-static_assert(128 * kRegsCtrl + 32 * kEpiWarps * kRegsEpi + 128 * kGroups * kRegsConv + 32 * kLoadWarps * kRegsLoad <= 64 * kManyThreads, "shares of the registers");
+constexpr int kConvGroups = 2;
+constexpr int kFirstEpi = 4, kEpiWarps = 8, kFirstConv = kFirstEpi + kEpiWarps, kFirstLoad = kFirstConv + 4 * kConvGroups, kLoadWarps = 4;
+constexpr int kManyThreads = 32 * (kFirstLoad + kLoadWarps);   // 768: launched with 80 registers a thread
+constexpr uint32_t kRegsCtrl = 40, kRegsEpi = 136, kRegsConv = 64, kRegsLoad = 40;
+static_assert(128 * kRegsCtrl + 32 * kEpiWarps * kRegsEpi + 128 * kConvGroups * kRegsConv + 32 * kLoadWarps * kRegsLoad <= 80 * kManyThreads, "shares of the registers");
 constexpr int kMaxRaw = 12, kMaxSlots = 8, kMaxAcc = 2;
 __host__ __device__ constexpr uint32_t slots(int ks) { return ks == 128 ? 4 : 6; }   // steps under way, in 256 columns at most
 constexpr uint32_t kTmemCols = 512;
@@ -58,7 +58,16 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void cp_async_wait_but2() { asm volatile("cp.async.wait_group 2;" ::: "memory"); }
 
-struct Strip { uint32_t expert, row0, rows, height, n0; };   // n0: of this CTA's 128 channels
+// Two fp32 sums at a time.
+__device__ __forceinline__ uint64_t pack_u32x2(uint32_t lo, uint32_t hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+    return d;
+}
+__device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) { return pack_u32x2(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ void fma_f32x2(uint64_t& d, uint64_t a, uint64_t b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b)); }
+
+struct Strip : ExpertStrip { uint32_t n0; };   // n0: of this CTA's 128 channels
 
 template <int BITS, bool GROUPED, int KS>
 __global__ void __launch_bounds__(kManyThreads, 1)
@@ -79,9 +88,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
     auto acc_empty = [&](uint32_t s) { return bar(2 * (kMaxRaw + kMaxSlots) + kMaxAcc + s); };   // rank 0: of both CTAs
     volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(smem_gen + kOffMisc);   // TMEM base, abort flag
     volatile uint32_t* abort_flag = misc + 1;
-    uint32_t* strips_before = reinterpret_cast<uint32_t*>(smem_gen + kOffTable);   // [experts + 1]
-    uint32_t* first_row = strips_before + p.x.experts + 1;                         // [experts]
-    uint32_t* row_count = first_row + p.x.experts;                                 // [experts]
+    const ExpertTable table(smem_gen + kOffTable, p.x.experts);
     const uint32_t act_stride = p.x.tile_rows * KS;   // bytes of one CTA's half of a step, at most
     const uint32_t off_act = p.off_raw + p.raw_stages * kRawBytes;
 
@@ -100,27 +107,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
         ptx::tmem_alloc_pair(ptx::smem_u32(const_cast<uint32_t*>(misc)), kTmemCols);
         ptx::tmem_relinquish_pair();
     }
-    if (warp == 3) {   // the table: 32 experts at a time
-        uint32_t before = 0;
-        for (uint32_t e0 = 0; e0 < p.x.experts; e0 += 32) {
-            const uint32_t e = e0 + lane;
-            uint32_t lo = 0, hi = 0;
-            if (e < p.x.experts) {
-                lo = clamp_offset(__ldg(p.x.offsets + e), p.x.m);
-                hi = max(lo, clamp_offset(__ldg(p.x.offsets + e + 1), p.x.m));
-            }
-            const uint32_t mine = (hi - lo + p.x.tile_rows - 1) / p.x.tile_rows;
-            uint32_t upto = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += y;
-            }
-            if (e < p.x.experts) { strips_before[e] = before + upto - mine; first_row[e] = lo; row_count[e] = hi - lo; }
-            before += __shfl_sync(0xffffffffu, upto, 31);
-        }
-        if (lane == 0) strips_before[p.x.experts] = before;
-    }
+    if (warp == 3) table.build(p.x, lane);
     __syncwarp();
     ptx::tc_fence_before_sync();
     __syncthreads();       // the table
@@ -134,23 +121,12 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
     auto give_up = [&](int where, uint32_t a, uint32_t b) {
         if (!*abort_flag) { report_timeout(p.status, where, (int)a, (int)b); *abort_flag = 1; }
     };
-    const uint32_t tiles = strips_before[p.x.experts] * p.x.n_blocks;   // < 2^31, the launcher sees to it
+    const uint32_t tiles = table.strips() * p.x.n_blocks;   // < 2^31, the launcher sees to it
     uint32_t t = worker;   // every role of both CTAs walks the same list of tiles
     auto next = [&](Strip& s) {
         if (t >= tiles) return false;
-        const uint32_t q = t / p.x.n_blocks;
-        uint32_t lo = 0, hi = p.x.experts;   // the expert with strips_before[e] <= q < strips_before[e + 1]
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (strips_before[mid] <= q) lo = mid; else hi = mid;
-        }
-        const uint32_t first = strips_before[lo], of = strips_before[lo + 1] - first, r = t - first * p.x.n_blocks, nt = r / of, i = r - nt * of;
-        const uint32_t all = row_count[lo], height = ((all + of - 1) / of + kUnit - 1) / kUnit * kUnit;
-        s.expert = lo;
-        s.height = height;
-        s.row0 = first_row[lo] + i * height;
-        s.rows = i * height < all ? min(height, all - i * height) : 0u;
-        s.n0 = (2 * nt + rank) * kCh;
+        table.tile(p.x, t, kUnit, s);
+        s.n0 = (2 * s.block + rank) * kCh;
         t += workers;
         return true;
     };
@@ -243,11 +219,11 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
             const uint32_t nn = x.n0 + ch;
             const size_t chan = (size_t)x.expert * p.x.n + (nn < p.x.n ? nn : 0);
             if (!GROUPED && has_zero) add = zero_add(chan);
-            uint32_t l = (g - steps_before) & (kGroups - 1);
+            uint32_t l = (g - steps_before) & (kConvGroups - 1);
             Ring rr, rs;
             rr.set(blocks_before + l / SPB, p.raw_stages);
             rs.set(steps_before + l, kSlots);
-            for (; l < ns; l += kGroups) {
+            for (; l < ns; l += kConvGroups) {
                 const uint32_t sub = l % SPB;
                 if (GROUPED && has_zero) add = zero_add(chan * groups_per_row + ((l * KS) >> p.x.group_shift));
                 if (p.slot_first && !warp_wait(step_empty(rs.i), rs.phase ^ 1u, abort_flag)) { give_up(66, x.expert, l); ok = false; break; }
@@ -294,8 +270,8 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                     const uint32_t left = ns - (l - sub);   // steps of this block and all after it
                     ptx::mbar_arrive_count(raw_empty(rr.i), left < SPB && sub + 1 == left ? 1 + SPB - left : 1u);   // a short last block: for its missing steps, too
                 }
-                rr.step(kGroups / SPB, p.raw_stages);   // four steps on
-                rs.step(kGroups, kSlots);
+                rr.step((sub + kConvGroups) / SPB, p.raw_stages);   // of this group's next step
+                rs.step(kConvGroups, kSlots);
             }
             steps_before += ns;
             blocks_before += (ns + SPB - 1) / SPB;
@@ -319,12 +295,11 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
         };
         while (ok && next(x)) {
             const uint32_t act_rows = x.height / 2, slab_bytes = act_rows * 128u;   // act_rows: a multiple of 16
-            const uint16_t* src[8];
+            uint32_t src[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {   // rows behind the last one, and those that A does not have: zeros
                 const uint32_t r0 = 16u * i + r8, c = rank * act_rows + r0;
-                const uint32_t row = r0 < act_rows && c < x.rows ? source_row(p.x, x.row0 + c) : 0xffffffffu;
-                src[i] = row < p.x.a_rows ? p.x.a + (size_t)row * p.x.lda + piece * 8u : nullptr;
+                src[i] = r0 < act_rows && c < x.rows ? source_row(p.x, x.row0 + c) : 0xffffffffu;
             }
             for (uint32_t l = 0; l < ns; ++l) {
                 // a free slot: go on; otherwise first report all that is under way
@@ -333,12 +308,14 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                     if (!warp_wait(step_empty(r.i), r.phase ^ 1u, abort_flag)) { give_up(62, x.expert, l); ok = false; break; }
                 }
                 const uint32_t to = at + r.i * act_stride;
+                const uint16_t* from = p.x.a + l * KS + piece * 8u;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     if (16u * i >= act_rows) break;
+                    const bool there = src[i] < p.x.a_rows;
+                    const uint16_t* row = there ? from + (size_t)src[i] * p.x.lda : p.x.a;
 #pragma unroll
-                    for (int h = 0; h < KS / kSlab; ++h)
-                        cp_async16_or_zero(to + h * slab_bytes + i * 2048u, src[i] ? (const void*)(src[i] + (size_t)l * KS + h * kSlab) : (const void*)p.x.a, src[i] != nullptr);
+                    for (int h = 0; h < KS / kSlab; ++h) cp_async16_or_zero(to + h * slab_bytes + i * 2048u, row + (there ? h * kSlab : 0), there);
                 }
                 cp_async_commit();
                 ++pending;
@@ -397,41 +374,58 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
             };
             const uint32_t column = tmem_base + ((quarter * 32u) << 16) + half * cols;
             if (GROUPED) {
-                float sum[kPacks][16];
+                uint64_t sum[kPacks][8];   // two rows each
 #pragma unroll
                 for (int i = 0; i < kPacks; ++i)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) sum[i][j] = 0.f;
-                auto group_scale = [&](uint32_t l) {
-                    if (l >= ns) return 0.f;
-                    const size_t i = chan * groups_per_row + ((l * KS) >> p.x.group_shift);
-                    return p.x.scale_dtype == AFB_SCALE_BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.x.scale)[i] << 16)
-                                                             : reinterpret_cast<const float*>(p.x.scale)[i];
+                    for (int j = 0; j < 8; ++j) sum[i][j] = 0;
+                // scales of four steps at a time, fetched while those of the four before are used: one fetched per step was waited for
+                const bool half_scale = p.x.scale_dtype == AFB_SCALE_BF16;
+                const size_t scale0 = chan * groups_per_row;
+                auto group_scale = [&](uint32_t l) -> uint32_t {
+                    if (l >= ns) return 0u;
+                    const size_t i = scale0 + ((l * KS) >> p.x.group_shift);
+                    return half_scale ? reinterpret_cast<const uint16_t*>(p.x.scale)[i] : reinterpret_cast<const uint32_t*>(p.x.scale)[i];
                 };
-                float sc = group_scale(0);
-                for (uint32_t l = 0; l < ns; ++l) {
-                    const float sc_nxt = group_scale(l + 1);
-                    if (!warp_wait(acc_full(rc.i), rc.phase, abort_flag)) { give_up(68, x.expert, l); ok = false; break; }
-                    ptx::tc_fence_after_sync();
+                uint32_t ahead[4];
 #pragma unroll
-                    for (int i = 0; i < kPacks; ++i) {
-                        if (16u * i >= cols) break;
-                        uint32_t a[16];
-                        ptx::tmem_ld_32x16(column + rc.i * acc_cols + 16 * i, a);
-                        ptx::tmem_ld_wait();
-                        if (16u * (i + 1) >= cols) drained();
+                for (int i = 0; i < 4; ++i) ahead[i] = group_scale(i);
+                for (uint32_t l = 0; l < ns; l += 4) {
+                    uint32_t now[4];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) sum[i][j] = fmaf(sc, __uint_as_float(a[j]), sum[i][j]);
+                    for (int i = 0; i < 4; ++i) { now[i] = ahead[i]; ahead[i] = group_scale(l + 4 + i); }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        if (l + u >= ns) break;
+                        const float sc = __uint_as_float(half_scale ? now[u] << 16 : now[u]);
+                        if (!warp_wait(acc_full(rc.i), rc.phase, abort_flag)) { give_up(68, x.expert, l); ok = false; break; }
+                        ptx::tc_fence_after_sync();
+                        const uint32_t from = column + rc.i * acc_cols;
+                        const uint64_t sc2 = pack_f32x2(sc, sc);
+#pragma unroll
+                        for (int i = 0; i < kPacks; ++i) {
+                            if (16u * i >= cols) break;
+                            uint32_t a[16];
+                            ptx::tmem_ld_32x16(from + 16 * i, a);
+                            ptx::tmem_ld_wait();
+                            if (16u * (i + 1) >= cols) drained();
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) fma_f32x2(sum[i][j], sc2, pack_u32x2(a[2 * j], a[2 * j + 1]));
+                        }
+                        rc.step(1, 2);
                     }
-                    rc.step(1, 2);
-                    sc = sc_nxt;
+                    if (!ok) break;
                 }
                 if (!ok) break;
 #pragma unroll
                 for (int i = 0; i < kPacks; ++i) {
+                    float v[16];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) sum[i][j] *= kUnpackInverse;
-                    finish(o[i], sum[i]);
+                    for (int j = 0; j < 8; ++j) {
+                        v[2 * j] = __uint_as_float((uint32_t)sum[i][j]) * kUnpackInverse;
+                        v[2 * j + 1] = __uint_as_float((uint32_t)(sum[i][j] >> 32)) * kUnpackInverse;
+                    }
+                    finish(o[i], v);
                 }
             } else {
                 const float scale = p.x.scale_dtype == AFB_SCALE_BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.x.scale)[chan] << 16)
@@ -546,15 +540,15 @@ int launch_expert_many(const ExpertParams& q, uint32_t bits, uint32_t group, Dev
     p.x.n_blocks = (q.n + 2 * kCh - 1) / (2 * kCh);
     p.steps = q.k / ks;
     p.accs = p.x.tile_rows <= 128 ? 2 : 1;
-    p.off_raw = (kOffTable + (3 * q.experts + 1) * (uint32_t)sizeof(uint32_t) + 1023u) / 1024u * 1024u;
+    p.off_raw = (kOffTable + ExpertTable::bytes(q.experts) + 1023u) / 1024u * 1024u;
     const uint32_t act_bytes = kSlots * p.x.tile_rows * ks;
     p.raw_stages = (232448 - 1024 - p.off_raw - act_bytes) / kRawBytes;
     if (p.raw_stages > (uint32_t)kMaxRaw) p.raw_stages = kMaxRaw;
-    // The parity waits of the converters (stream.cu): a converter warp sees every fourth step only, and its wait for phase n of a raw block means
+    // The parity waits of the converters (stream.cu): a converter warp sees every second step only, and its wait for phase n of a raw block means
     // something once phase n - 1 is complete.  A free slot says that the step kSlots back has been multiplied and so, with one issuing warp, all
     // before it.  With two, the other one may be a step behind: its last but one has been, since the accumulators are drained in order.
     const uint32_t back = kSlots + (group ? 2 : 0), per_block = p.steps % spb == 0 ? spb : 1;
-    p.slot_first = p.raw_stages * per_block >= kGroups + back + per_block - 1 ? 0u : 1u;
+    p.slot_first = p.raw_stages * per_block >= kConvGroups + back + per_block - 1 ? 0u : 1u;
     if (p.raw_stages * per_block < back + per_block - 1) return AFB_ERR_UNSUPPORTED;   // not with any size that this function takes
     p.c_vec = q.ldc % 8 == 0 && (uintptr_t)q.c % 16 == 0 && q.n_out % 8 == 0;
     p.status = ctx->status;
