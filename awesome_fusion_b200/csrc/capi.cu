@@ -20,6 +20,7 @@ constexpr size_t kSplitKWorkspaceBytes = 32u << 20;
 constexpr size_t kSplitKCounters = 4096;
 constexpr int kPreallocatedWorkspaces = 8;
 constexpr size_t kMinStreamWorkspace = 4u << 20;       // of a captured graph: a power of two from here on
+constexpr size_t kMaxStreamWorkspace = 1024u << 20;
 constexpr size_t kMaxStreamWorkspaceTotal = 3072u << 20;   // 79 streams of 148 SMs; beyond this, and beyond kMaxStreamWorkspaces, launches take another form
 // Captured graphs whose workspaces stay theirs until afb_finalize, as streams' do.  Those of further graphs go back to the pool when the
 // graph is gone; the user object that says so costs each replay of the graph 2.5 us (16 x 22016 x 4096 int4, captured: 30.9 / 33.9 us).
@@ -124,9 +125,10 @@ bool stream_workspace(DeviceCtx* ctx, cudaStream_t s, size_t bytes, float** ws, 
     std::lock_guard<std::mutex> lock(g_mutex);
     // a stream's own workspace serves all its launches to come, a graph's the one at hand and those no larger
     const size_t whole = stream_workspace_bytes(ctx->sm_count);
-    if (bytes > whole) return false;
+    if (bytes > kMaxStreamWorkspace) return false;
     size_t want = whole;
-    if (capturing) for (want = kMinStreamWorkspace; want < bytes;) want = want * 2 < whole ? want * 2 : whole;
+    if (bytes > whole) while (want < bytes) want *= 2;   // the converted activations of products grouped by expert
+    else if (capturing) for (want = kMinStreamWorkspace; want < bytes;) want = want * 2 < whole ? want * 2 : whole;
     DeviceCtx::StreamWorkspace* spare = nullptr;   // smallest one with memory that is large enough
     DeviceCtx::StreamWorkspace* empty = nullptr;
     for (auto& w : ctx->stream_workspaces) {

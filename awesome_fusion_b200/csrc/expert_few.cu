@@ -391,6 +391,10 @@ extern "C" int afb_expert_gemm_launch(const afb_expert_gemm_args* x, void* strea
     for (uint32_t g = a.group_size; g > 1; g >>= 1) ++p.group_shift;
     p.gated = x->gated; p.silu = x->activation == AFB_ACT_SILU ? 1u : 0u;
     const bool many = a.variant == AFB_VARIANT_PREFILL || (a.variant == AFB_VARIANT_AUTO && (uint64_t)a.m > 24ull * x->experts);
-    if (many && x->a_rows) return launch_expert_many(p, a.b_bits, a.group_size, ctx, (cudaStream_t)stream);
+    if (many && x->a_rows) {
+        bool done = false;
+        const int rc = launch_expert_many(p, a.b_bits, a.group_size, ctx, (cudaStream_t)stream, &done);
+        if (done) return rc;
+    }
     return launch_expert_few(p, a.b_bits, a.group_size, ctx, (cudaStream_t)stream);
 }

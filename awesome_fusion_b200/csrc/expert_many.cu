@@ -6,19 +6,22 @@
 // one tcgen05.mma.cta_group::2 reads both halves.  An expert's rows are cut into strips of equal height, a multiple of 32.
 //
 //   warp 0        TMA: raw weight blocks, 128 channels x 128 bytes, 128-byte swizzle
-//   warps 2, 3    rank 0: tcgen05.mma 256 x height x 16;  rank 1, warp 2: reports to rank 0 that its half of a step is complete
+//   warp 2        rank 0: tcgen05.mma 256 x height x 16;  rank 1: reports to rank 0 that its half of a step is complete
 //   warps 4-11    epilogue, two per lane quarter: accumulator -> registers -> (accumulator free) -> shared memory -> C
 //   warps 12-19   converters: two groups of four warps; group g takes every second step of k (KS = 128 or 64 wide)
 //   warps 20-23   the rows of A: 16-byte copies to shared memory, written in the 128-byte swizzle.  (A TMA gather of four rows takes 65 cycles of
 //                 the issuing warp, which has to make every lane's row numbers uniform first: 4200 cycles per step of 256 rows.)
 //
-// Scales per channel: the sum over all of K stays in the accumulator, strips of up to 256 rows.
-// Scales per group: a weight times its scale has no room in a bf16 (up to 8 x 8 significant bits), and rounding it there costs as much
-// accuracy as the rounding of the result.  So every step has an accumulator of its own, two take turns, and the epilogue warps add scale * sum in
-// fp32 registers: strips of up to 128 rows (64 sums a thread).  A step is then 512 cycles of tensor work, less than one warp needs to issue it
-// (wait 80, eight MMAs 480, two commits 360): two warps issue, one per accumulator.
+// The sum over all of K stays in the accumulator.  Scales per channel multiply it in the end.  Scales per group go into the weights, and there bf16 has no
+// room for them: a weight of 4 bits times a scale of 8 has up to 12 significant ones, and a rounding to 8 costs as much accuracy as the rounding of the
+// result.  So these products are made in fp16, with 11: int4 without zero-points exactly (|q| <= 8 has three significant bits), with them and int8 off by
+// 2^-11 at most.  What fp16 lacks is range, so a kernel ahead of this one gives every row of A a power of two that brings its largest value below 2^15 (what is
+// below 2^-28 of it loses bits: 2^-40 of the largest at most), and finds one for every channel's scales (below 2^-20 of the largest they lose bits); the
+// epilogue takes both out again.  (Tried before: sums of each group in accumulators of their own, scaled and added in fp32 registers, which is exact, too:
+// 1650 cycles per step of 128 rows, the chain from accumulator to registers and back; 2048 tokens, 64 experts of 2048 x 4096 int4: 516 us.)
 //
 // Every role walks the same tiles (ExpertTable): worker, worker + workers, ...
+#include <cuda_fp16.h>
 #include "dequant.cuh"
 #include "expert_common.cuh"
 #include "stream_common.cuh"
@@ -48,6 +51,8 @@ struct ManyParams {
     uint32_t slot_first;      // converters wait for their slot before they wait for their raw block
     uint32_t off_raw;         // behind the table
     uint32_t c_vec;           // 16-byte stores of C
+    const float* row_factor;    // group scales: see PrepareParams
+    const float* channel_mult;
     int32_t* status;
 };
 
@@ -58,14 +63,87 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void cp_async_wait_but2() { asm volatile("cp.async.wait_group 2;" ::: "memory"); }
 
-// Two fp32 sums at a time.
-__device__ __forceinline__ uint64_t pack_u32x2(uint32_t lo, uint32_t hi) {
-    uint64_t d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+// Two fp16 values at a time.
+__device__ __forceinline__ uint32_t f16x2_mul(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
-__device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) { return pack_u32x2(__float_as_uint(lo), __float_as_uint(hi)); }
-__device__ __forceinline__ void fma_f32x2(uint64_t& d, uint64_t a, uint64_t b) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b)); }
+__device__ __forceinline__ uint32_t f16x2_fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t f16_dup(float v) { return (uint32_t)__half_as_ushort(__float2half_rn(v)) * 0x00010001u; }
+// The largest power of two that is not above v, as its exponent; 0 for v = 0, infinity and NaN.
+__device__ __forceinline__ int exponent_of(float v) {
+    const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
+    if (u == 0u || u >= 0x7f800000u) return 0;
+    return u >= 0x00800000u ? (int)(u >> 23) - 127 : -118 - __clz((int)u);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
+// The factor that brings values of up to 2^(e + 1) below 2^15.
+__device__ __forceinline__ int headroom(int e) { return min(14 - e, 126); }
+
+// Group scales: the rows of A as fp16 with a power of two of their own, and the power of two of each channel's scales.  A warp takes a row, the
+// warps after them 32 channels each (of experts that have rows).
+struct PrepareParams {
+    ExpertParams x;
+    uint16_t* a;          // [a_rows, k]
+    float* row_factor;    // what a row's products have to be multiplied by
+    float* channel_mult;  // [experts * n] what a channel's scales are multiplied by
+};
+constexpr int kPrepareThreads = 256;
+__global__ void __launch_bounds__(kPrepareThreads) expert_prepare_kernel(const PrepareParams p) {
+    const uint32_t lane = threadIdx.x & 31, id = blockIdx.x * (kPrepareThreads / 32) + (threadIdx.x >> 5);
+    if (id < p.x.a_rows) {
+        const uint16_t* src = p.x.a + (size_t)id * p.x.lda;
+        uint32_t most = 0;
+#pragma unroll 4
+        for (uint32_t c = lane * 8; c < p.x.k; c += 256) {
+            const uint4 v = *reinterpret_cast<const uint4*>(src + c);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t a = (w[i] >> (16 * h)) & 0x7fffu;
+                    if (a < 0x7f80u) most = max(most, a);   // infinities and NaN stay what they are
+                }
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        const int e = headroom(exponent_of(__uint_as_float(most << 16)));
+        const float mult = power_of_two(e);
+        uint16_t* dst = p.a + (size_t)id * p.x.k;
+#pragma unroll 4
+        for (uint32_t c = lane * 8; c < p.x.k; c += 256) {
+            const uint4 v = *reinterpret_cast<const uint4*>(src + c);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            uint32_t o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __half2 h = __floats2half2_rn(__uint_as_float(w[i] << 16) * mult, __uint_as_float(w[i] & 0xffff0000u) * mult);
+                o[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            *reinterpret_cast<uint4*>(dst + c) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        if (lane == 0) p.row_factor[id] = power_of_two(-e);
+        return;
+    }
+    const uint64_t chan = (uint64_t)(id - p.x.a_rows) * 32 + lane, channels = (uint64_t)p.x.experts * p.x.n;
+    if (chan >= channels) return;
+    const uint32_t expert = (uint32_t)(chan / p.x.n);
+    if (clamp_offset(__ldg(p.x.offsets + expert + 1), p.x.m) <= clamp_offset(__ldg(p.x.offsets + expert), p.x.m)) return;
+    const uint32_t groups = p.x.k >> p.x.group_shift;
+    float most = 0.f;
+#pragma unroll 8
+    for (uint32_t g = 0; g < groups; ++g) {
+        const float s = fabsf(p.x.scale_dtype == AFB_SCALE_BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.x.scale)[chan * groups + g] << 16)
+                                                                : reinterpret_cast<const float*>(p.x.scale)[chan * groups + g]);
+        if (s < INFINITY) most = fmaxf(most, s);
+    }
+    p.channel_mult[chan] = power_of_two(headroom(exponent_of(most)));
+}
 
 struct Strip : ExpertStrip { uint32_t n0; };   // n0: of this CTA's 128 channels
 
@@ -75,7 +153,6 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
     constexpr uint32_t SPB = (BITS == 8 ? 128 : 256) / KS;   // steps per raw block
     constexpr uint32_t kSlotCols = KS / 2;                   // TMEM columns of a step's weights
     constexpr uint32_t kSlots = slots(KS);
-    constexpr uint32_t kIssuers = GROUPED ? 2 : 1;
     extern __shared__ uint8_t smem_raw_base[];
     const uint32_t smem_base = (ptx::smem_u32(smem_raw_base) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw_base + (smem_base - ptx::smem_u32(smem_raw_base));
@@ -156,37 +233,31 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
             }
             for (uint32_t s = 0; s < p.raw_stages; ++s)   // never leave with a bulk copy still writing this CTA's shared memory
                 if (issued & (1u << s)) ptx::mbar_wait(raw_full(s), (parity >> s) & 1u);
-        } else if (rank == 0 && (uint32_t)warp - 2 < kIssuers) {
-            // ======================= MMA issuers: every kIssuers-th step =======================
-            const uint32_t who = (uint32_t)warp - 2;
+        } else if (warp == 2 && rank == 0) {
+            // ======================= MMA issuer =======================
             const uint64_t desc0 = ptx::umma_desc_kmajor_sw128(smem_base + off_act);
-            r.i = who;
-            Ring rc{who, 0};
+            Ring rc{0, 0};
             bool ready = false;
-            uint32_t before = 0, g = who;   // steps of the tiles walked so far; this warp's next step, counted over all tiles
             while (ok && next(x)) {
-                const uint32_t idesc = ptx::umma_idesc_bf16_f32(2 * kCh, x.height), slab_d = x.height * 64u >> 4;
-                if (!GROUPED && !warp_wait(acc_empty(rc.i), rc.phase ^ 1u, abort_flag)) { give_up(63, x.expert, 0); break; }
-                for (; g < before + ns; g += kIssuers) {
-                    if (GROUPED && !warp_wait(acc_empty(who), rc.phase ^ 1u, abort_flag)) { give_up(63, x.expert, g); ok = false; break; }
-                    if (!__all_sync(0xffffffffu, ready) && !warp_wait(step_full(r.i), r.phase, abort_flag)) { give_up(64, x.expert, g); ok = false; break; }
+                const uint32_t idesc = GROUPED ? ptx::umma_idesc_f16_f32(2 * kCh, x.height) : ptx::umma_idesc_bf16_f32(2 * kCh, x.height), slab_d = x.height * 64u >> 4;
+                const uint32_t td = tmem_base + rc.i * acc_cols, acc_done = acc_full(rc.i);
+                if (!warp_wait(acc_empty(rc.i), rc.phase ^ 1u, abort_flag)) { give_up(63, x.expert, 0); break; }
+                rc.step(1, p.accs);
+                for (uint32_t l = 0; l < ns; ++l) {
+                    if (!__all_sync(0xffffffffu, ready) && !warp_wait(step_full(r.i), r.phase, abort_flag)) { give_up(64, x.expert, l); ok = false; break; }
                     ptx::tc_fence_after_sync();
-                    const uint32_t ta = slot_base + r.i * kSlotCols, td = tmem_base + rc.i * acc_cols, done = step_empty(r.i), acc_done = acc_full(rc.i);
+                    const uint32_t ta = slot_base + r.i * kSlotCols, done = step_empty(r.i);
                     const uint64_t db = desc0 + r.i * (act_stride >> 4);
-                    const bool first = GROUPED || g == before, last = GROUPED || g + 1 == before + ns;
-                    r.step(kIssuers, kSlots);
+                    r.step(1, kSlots);
                     ready = ptx::mbar_test_wait(step_full(r.i), r.phase);   // of the next step: the answer is back when this one has been issued
                     if (ptx::elect_one()) {
 #pragma unroll
                         for (int j = 0; j < KS / 16; ++j)
-                            ptx::umma_bf16_ts_pair(td, ta + 8 * j, db + (uint32_t)(j / 4) * slab_d + 2u * (j % 4), idesc, !first || j > 0 ? 1u : 0u);
+                            ptx::umma_bf16_ts_pair(td, ta + 8 * j, db + (uint32_t)(j / 4) * slab_d + 2u * (j % 4), idesc, l > 0 || j > 0 ? 1u : 0u);   // kind::f16: the types are the descriptor's
                         ptx::umma_commit_pair(done);
-                        if (last) ptx::umma_commit_pair(acc_done);
+                        if (l + 1 == ns) ptx::umma_commit_pair(acc_done);
                     }
-                    if (GROUPED) rc.phase ^= 1u;
                 }
-                before += ns;
-                if (!GROUPED) rc.step(1, p.accs);
             }
         } else if (warp == 2) {
             // ======================= rank 1: reports its half of each step =======================
@@ -210,22 +281,44 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
         const Nibbles nib = nibbles(p.x.packed != 0);
         const bool has_zero = p.x.zero != nullptr;
         const uint32_t groups_per_row = GROUPED ? p.x.k >> p.x.group_shift : 0;
-        auto zero_add = [&](size_t i) { return unpack_add(BITS, BITS == 8 ? decode_zero8(p.x.zero[i], p.x.enc) : decode_zero4(p.x.zero[i], p.x.enc)); };
-        uint32_t add = unpack_add(BITS, 0);
+        auto zero_of = [&](size_t i) { return BITS == 8 ? decode_zero8(p.x.zero[i], p.x.enc) : decode_zero4(p.x.zero[i], p.x.enc); };
+        // bf16: weight * 2^-6 in one step (dequant.cuh).  fp16: an unsigned weight u, zero-extended, is u * 2^-24; fma makes (u - 128 - zero) * 2^-9 of it,
+        // exactly, and a multiplication by the channel's scale, at most 2^15, rounds once.
+        constexpr uint32_t kByteF16 = 0x78007800u, kHighF16 = 0x68006800u, kPairF16 = 0x68007800u;   // 2^15, 2^11, 2^11 and 2^15
+        auto add_of = [&](int zero) { return GROUPED ? f16_dup((float)(-(BITS == 8 ? 128 : 8) - zero) * 0x1p-9f) : unpack_add(BITS, zero); };
+        const uint32_t mul0 = BITS == 8 ? (GROUPED ? kByteF16 : kMulByte) : !GROUPED ? nib.mul[0] : p.x.packed ? kByteF16 : kPairF16;
+        const uint32_t mul1 = BITS == 8 ? mul0 : !GROUPED ? nib.mul[1] : p.x.packed ? kHighF16 : kPairF16;
+        auto unpack2 = [&](uint32_t v, uint32_t mul, uint32_t add, uint32_t sc) { return GROUPED ? f16x2_mul(f16x2_fma(v, mul, add), sc) : bf16x2_fma(v, mul, add); };
+        uint32_t add = add_of(0);
         const uint32_t row = p.off_raw + ch * 128, swz = (ch & 7u) << 4, lanes = (quarter * 32u) << 16;
         uint32_t steps_before = 0, blocks_before = 0;   // of the tiles walked so far
         bool ok = true;
         while (ok && next(x)) {
             const uint32_t nn = x.n0 + ch;
             const size_t chan = (size_t)x.expert * p.x.n + (nn < p.x.n ? nn : 0);
-            if (!GROUPED && has_zero) add = zero_add(chan);
+            if (!GROUPED && has_zero) add = add_of(zero_of(chan));
+            const float mult = GROUPED ? p.channel_mult[chan] : 1.f;
+            // scale and zero-point of this group's next step, as they are stored
+            uint32_t sc_nxt = 0, z_nxt = 0;
+            auto load_group = [&](uint32_t l) {
+                if (!GROUPED || l >= ns) return;
+                const size_t i = chan * groups_per_row + ((l * KS) >> p.x.group_shift);
+                sc_nxt = p.x.scale_dtype == AFB_SCALE_BF16 ? reinterpret_cast<const uint16_t*>(p.x.scale)[i] : reinterpret_cast<const uint32_t*>(p.x.scale)[i];
+                if (has_zero) z_nxt = p.x.zero[i];
+            };
             uint32_t l = (g - steps_before) & (kConvGroups - 1);
             Ring rr, rs;
             rr.set(blocks_before + l / SPB, p.raw_stages);
             rs.set(steps_before + l, kSlots);
+            load_group(l);
             for (; l < ns; l += kConvGroups) {
                 const uint32_t sub = l % SPB;
-                if (GROUPED && has_zero) add = zero_add(chan * groups_per_row + ((l * KS) >> p.x.group_shift));
+                uint32_t sc = 0;
+                if (GROUPED) {
+                    sc = f16_dup(__uint_as_float(p.x.scale_dtype == AFB_SCALE_BF16 ? sc_nxt << 16 : sc_nxt) * mult);
+                    if (has_zero) add = add_of(BITS == 8 ? decode_zero8(z_nxt, p.x.enc) : decode_zero4(z_nxt, p.x.enc));
+                    load_group(l + kConvGroups);
+                }
                 if (p.slot_first && !warp_wait(step_empty(rs.i), rs.phase ^ 1u, abort_flag)) { give_up(66, x.expert, l); ok = false; break; }
                 if (!warp_wait(raw_full(rr.i), rr.phase, abort_flag)) { give_up(67, x.expert, l); ok = false; break; }
                 const uint32_t raw = smem_base + row + rr.i * kRawBytes, slot = slot_base + lanes + rs.i * kSlotCols;
@@ -246,11 +339,13 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                         for (int j = 0; j < kPerStore; ++j) {
                             const uint32_t v = w[q * kPerStore + j];
                             if (BITS == 8) {
-                                s8x4_to_bf16(v, flip, sel0, sel1, kMulByte, add, o[2 * j], o[2 * j + 1]);
-                            } else {
-                                uint32_t qv[4];
-                                s4x8_to_bf16(v, flip, nib, nib.mul[0], nib.mul[1], add, qv);
-                                o[4 * j] = qv[0]; o[4 * j + 1] = qv[1]; o[4 * j + 2] = qv[2]; o[4 * j + 3] = qv[3];
+                                const uint32_t t8 = v ^ flip;
+                                o[2 * j] = unpack2(prmt(t8, 0u, sel0), mul0, add, sc);
+                                o[2 * j + 1] = unpack2(prmt(t8, 0u, sel1), mul0, add, sc);
+                            } else {   // s4x8_to_bf16's steps
+                                const uint32_t e = lop3_and_xor(v, 0x0f0f0f0fu, flip & 0x0f0f0f0fu), d = lop3_and_xor(v, 0xf0f0f0f0u, flip & 0xf0f0f0f0u);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) o[4 * j + i] = unpack2(prmt(e, d, nib.sel[i]), i % 2 ? mul1 : mul0, add, sc);
                             }
                         }
                         if (h == 0 && q == 0) {
@@ -332,10 +427,9 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
         // ======================= epilogue =======================
         ptx::regs_up<kRegsEpi>();
         const uint32_t quarter = (uint32_t)warp & 3u, half = (uint32_t)(warp - kFirstEpi) >> 2, ch = quarter * 32 + lane;
-        constexpr int kPacks = GROUPED ? 4 : 8;   // of 16 columns: this warp's half of a strip
+        constexpr int kPacks = 8;   // of 16 columns: this warp's half of a strip
         const bool odd = lane & 1, gated = p.x.gated != 0, act = p.x.silu != 0;
         const uint32_t stage = smem_base + kOffOut + (uint32_t)(warp - kFirstEpi) * 2 * kOutBytes;
-        const uint32_t groups_per_row = GROUPED ? p.x.k >> p.x.group_shift : 0;
         Ring rc{0, 0};
         bool ok = true;
         auto drained = [&] {   // everything of the accumulator is in registers
@@ -373,81 +467,34 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                 }
             };
             const uint32_t column = tmem_base + ((quarter * 32u) << 16) + half * cols;
-            if (GROUPED) {
-                uint64_t sum[kPacks][8];   // two rows each
-#pragma unroll
-                for (int i = 0; i < kPacks; ++i)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) sum[i][j] = 0;
-                // scales of four steps at a time, fetched while those of the four before are used: one fetched per step was waited for
-                const bool half_scale = p.x.scale_dtype == AFB_SCALE_BF16;
-                const size_t scale0 = chan * groups_per_row;
-                auto group_scale = [&](uint32_t l) -> uint32_t {
-                    if (l >= ns) return 0u;
-                    const size_t i = scale0 + ((l * KS) >> p.x.group_shift);
-                    return half_scale ? reinterpret_cast<const uint16_t*>(p.x.scale)[i] : reinterpret_cast<const uint32_t*>(p.x.scale)[i];
-                };
-                uint32_t ahead[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) ahead[i] = group_scale(i);
-                for (uint32_t l = 0; l < ns; l += 4) {
-                    uint32_t now[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) { now[i] = ahead[i]; ahead[i] = group_scale(l + 4 + i); }
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        if (l + u >= ns) break;
-                        const float sc = __uint_as_float(half_scale ? now[u] << 16 : now[u]);
-                        if (!warp_wait(acc_full(rc.i), rc.phase, abort_flag)) { give_up(68, x.expert, l); ok = false; break; }
-                        ptx::tc_fence_after_sync();
-                        const uint32_t from = column + rc.i * acc_cols;
-                        const uint64_t sc2 = pack_f32x2(sc, sc);
-#pragma unroll
-                        for (int i = 0; i < kPacks; ++i) {
-                            if (16u * i >= cols) break;
-                            uint32_t a[16];
-                            ptx::tmem_ld_32x16(from + 16 * i, a);
-                            ptx::tmem_ld_wait();
-                            if (16u * (i + 1) >= cols) drained();
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) fma_f32x2(sum[i][j], sc2, pack_u32x2(a[2 * j], a[2 * j + 1]));
-                        }
-                        rc.step(1, 2);
-                    }
-                    if (!ok) break;
-                }
-                if (!ok) break;
-#pragma unroll
-                for (int i = 0; i < kPacks; ++i) {
-                    float v[16];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        v[2 * j] = __uint_as_float((uint32_t)sum[i][j]) * kUnpackInverse;
-                        v[2 * j + 1] = __uint_as_float((uint32_t)(sum[i][j] >> 32)) * kUnpackInverse;
-                    }
-                    finish(o[i], v);
-                }
-            } else {
-                const float scale = p.x.scale_dtype == AFB_SCALE_BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.x.scale)[chan] << 16)
-                                                                      : reinterpret_cast<const float*>(p.x.scale)[chan];
-                if (!warp_wait(acc_full(rc.i), rc.phase, abort_flag)) { give_up(68, x.expert, 0); break; }
-                ptx::tc_fence_after_sync();
-#pragma unroll
-                for (int i = 0; i < kPacks; ++i) {
-                    if (16u * i >= cols) break;
-                    uint32_t a[16];
-                    float v[16];
-                    ptx::tmem_ld_32x16(column + rc.i * acc_cols + 16 * i, a);
-                    ptx::tmem_ld_wait();
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) v[j] = unscaled(__uint_as_float(a[j]), scale);
-                    finish(o[i], v);
-                }
-                drained();
-                rc.step(1, p.accs);
-            }
-            // Blocks of 16 rows turn round in shared memory and leave in 16-byte pieces, 64 (gated 32) contiguous bytes a row; two blocks take turns.
+            // Per channel the sum of products times the scale; of group scales the powers of two that channel and row were given.
             const uint32_t first = half * cols, valid = x.rows > first ? min(cols, x.rows - first) : 0u;
+            const float scale = GROUPED ? 1.f / p.channel_mult[chan]
+                                        : p.x.scale_dtype == AFB_SCALE_BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.x.scale)[chan] << 16)
+                                                                            : reinterpret_cast<const float*>(p.x.scale)[chan];
+            float factor[4];   // of rows lane, lane + 32, ...
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t row = i * 32 + lane < valid ? p.x.row_pair ? source_row(p.x, x.row0 + first + i * 32 + lane) : x.row0 + first + i * 32 + lane : 0xffffffffu;
+                factor[i] = GROUPED && row < p.x.a_rows ? p.row_factor[row] * 512.f : 0.f;
+            }
+            if (!warp_wait(acc_full(rc.i), rc.phase, abort_flag)) { give_up(68, x.expert, 0); break; }
+            ptx::tc_fence_after_sync();
+#pragma unroll
+            for (int i = 0; i < kPacks; ++i) {
+                if (16u * i >= cols) break;
+                uint32_t a[16];
+                float v[16];
+                ptx::tmem_ld_32x16(column + rc.i * acc_cols + 16 * i, a);
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    v[j] = GROUPED ? (__uint_as_float(a[j]) * scale) * __shfl_sync(0xffffffffu, factor[i / 2], i % 2 * 16 + j) : unscaled(__uint_as_float(a[j]), scale);
+                finish(o[i], v);
+            }
+            drained();
+            rc.step(1, p.accs);
+            // Blocks of 16 rows turn round in shared memory and leave in 16-byte pieces, 64 (gated 32) contiguous bytes a row; two blocks take turns.
             const uint32_t c0 = x.n0 + quarter * 32u;   // first channel of this warp
             if (c0 >= p.x.n) continue;
             uint16_t* c = p.x.c + (size_t)(x.row0 + first) * p.x.ldc;
@@ -531,12 +578,13 @@ int launch_cfg(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uint32
 
 }  // namespace
 
-int launch_expert_many(const ExpertParams& q, uint32_t bits, uint32_t group, DeviceCtx* ctx, cudaStream_t s) {
+int launch_expert_many(const ExpertParams& q, uint32_t bits, uint32_t group, DeviceCtx* ctx, cudaStream_t s, bool* done) {
+    *done = false;
     ManyParams p{};
     p.x = q;
     const uint32_t ks = q.k % 128 == 0 && group % 128 == 0 ? 128 : 64, spb = (bits == 8 ? 128 : 256) / ks, kSlots = slots(ks);
     // up to 128 rows there are two accumulators, and twice the raw blocks under way
-    p.x.tile_rows = group || (uint64_t)q.m <= 160ull * q.experts ? 128 : 256;
+    p.x.tile_rows = (uint64_t)q.m <= 160ull * q.experts ? 128 : 256;
     p.x.n_blocks = (q.n + 2 * kCh - 1) / (2 * kCh);
     p.steps = q.k / ks;
     p.accs = p.x.tile_rows <= 128 ? 2 : 1;
@@ -544,18 +592,36 @@ int launch_expert_many(const ExpertParams& q, uint32_t bits, uint32_t group, Dev
     const uint32_t act_bytes = kSlots * p.x.tile_rows * ks;
     p.raw_stages = (232448 - 1024 - p.off_raw - act_bytes) / kRawBytes;
     if (p.raw_stages > (uint32_t)kMaxRaw) p.raw_stages = kMaxRaw;
-    // The parity waits of the converters (stream.cu): a converter warp sees every second step only, and its wait for phase n of a raw block means
-    // something once phase n - 1 is complete.  A free slot says that the step kSlots back has been multiplied and so, with one issuing warp, all
-    // before it.  With two, the other one may be a step behind: its last but one has been, since the accumulators are drained in order.
-    const uint32_t back = kSlots + (group ? 2 : 0), per_block = p.steps % spb == 0 ? spb : 1;
-    p.slot_first = p.raw_stages * per_block >= kConvGroups + back + per_block - 1 ? 0u : 1u;
-    if (p.raw_stages * per_block < back + per_block - 1) return AFB_ERR_UNSUPPORTED;   // not with any size that this function takes
+    // the parity waits of the converters: see stream.cu
+    const uint32_t per_block = p.steps % spb == 0 ? spb : 1;
+    p.slot_first = p.raw_stages * per_block >= kConvGroups + kSlots + per_block - 1 ? 0u : 1u;
+    if (p.raw_stages * per_block < kSlots + per_block - 1) return AFB_ERR_UNSUPPORTED;   // not with any size that this function takes
     p.c_vec = q.ldc % 8 == 0 && (uintptr_t)q.c % 16 == 0 && q.n_out % 8 == 0;
     p.status = ctx->status;
     const uint64_t tiles = expert_tiles(q.m, q.experts, p.x.tile_rows) * p.x.n_blocks;
-    if (tiles >> 31) return AFB_ERR_TOO_LARGE;
+    if (tiles >> 31) { *done = true; return AFB_ERR_TOO_LARGE; }
     const uint32_t pairs = (uint32_t)ctx->sm_count / 2, grid = 2 * (tiles < pairs ? (uint32_t)tiles : pairs);
     const uint32_t smem = 1024 + p.off_raw + p.raw_stages * kRawBytes + act_bytes;
+    if (group) {
+        // rows of A, their factors, the channels' multipliers, each from a multiple of 256 bytes on
+        const uint64_t a_bytes = ((uint64_t)q.a_rows * q.k * 2 + 255) / 256 * 256, row_bytes = ((uint64_t)q.a_rows * 4 + 255) / 256 * 256;
+        const uint64_t channels = (uint64_t)q.experts * q.n, warps = q.a_rows + (channels + 31) / 32;
+        float* ws;
+        uint32_t* counters;
+        if (!stream_workspace(ctx, s, a_bytes + row_bytes + channels * 4, &ws, &counters)) return AFB_OK;
+        PrepareParams prep{};
+        prep.x = q;
+        prep.a = reinterpret_cast<uint16_t*>(ws);
+        prep.row_factor = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + a_bytes);
+        prep.channel_mult = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + a_bytes + row_bytes);
+        expert_prepare_kernel<<<(uint32_t)((warps + kPrepareThreads / 32 - 1) / (kPrepareThreads / 32)), kPrepareThreads, 0, s>>>(prep);
+        count_launch();
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) { *done = true; return cuda_fail(e); }
+        p.x.a = prep.a; p.x.lda = q.k;
+        p.row_factor = prep.row_factor; p.channel_mult = prep.channel_mult;
+    }
+    *done = true;
     CUtensorMap tw;
     const int rc = tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.b, (uint64_t)q.k * bits / 8, (uint64_t)q.experts * q.n, q.ldb_bytes, 128, kCh, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
