@@ -24,7 +24,8 @@ namespace {
 
 constexpr int kFewWarps = 16, kLoadWarps = 4, kFewThreads = 32 * (kFewWarps + kLoadWarps);   // 640: launched with 96 registers a thread
 constexpr uint32_t kRegsWork = 112, kRegsLoad = 32;
-static_assert(32 * kFewWarps * kRegsWork + 32 * kLoadWarps * kRegsLoad <= 96 * kFewThreads, "shares of the registers");
+constexpr uint32_t kRegsAll = 32 * kFewWarps * kRegsWork + 32 * kLoadWarps * kRegsLoad;
+static_assert(kRegsAll <= 96 * kFewThreads, "shares of the registers");
 constexpr uint32_t kWays = 4, kStages = 8;     // kStages: a multiple of kWays, so that a warp meets every phase of the stages that it meets
 constexpr uint32_t kHalfBytes = kCh * 64;      // a box of weights
 constexpr uint32_t kSumPitch = kCh + 4;        // floats per row of a way's sums
@@ -59,7 +60,10 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
 // Place of 16-byte piece `pc` of a row of A: the eight lanes that read at once hold two rows and, of int4, pieces 4 apart.
 __device__ __forceinline__ uint32_t act_place(uint32_t row, uint32_t pc) { return pc ^ (((pc >> 3) & 1u) << 1) ^ (row & 1u); }
 
-template <int BITS, int MT, bool GROUPED, bool HALF>
+template <int N> struct Tiles { static constexpr int value = N; };
+
+// PACKED (int4 only): the unpack of the pre-packed order, 9 instructions per 8 weights, with constants instead of registers; otherwise either order, 10.
+template <int BITS, int MT, bool GROUPED, bool HALF, bool PACKED>
 __global__ void __launch_bounds__(kFewThreads, 1)
 expert_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const FewParams p) {
     constexpr uint32_t CH = BITS == 8 ? 64 : 128, LK = CH / 4, AV = LK / 8;   // k per 64 bytes; of them per lane; 16-byte pieces of A per lane
@@ -158,6 +162,7 @@ expert_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const FewParams p)
         for (uint32_t i = blockIdx.x; i < tiles; i += gridDim.x) {
             table.tile(x, i, 1, t);
             const uint32_t n0 = t.block * kCh;
+            const bool two = MT > 1 && t.rows > 8;   // eight rows or less take one instruction where there could be two
             uint32_t chan[4];      // rows of B of this lane's channels: 8 apart
 #pragma unroll
             for (int j = 0; j < 4; ++j) chan[j] = t.expert * x.n + min(n0 + cg * 32 + j * 8 + g, x.n - 1);
@@ -168,6 +173,12 @@ expert_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const FewParams p)
             // scales and zero-points of this warp's next stage, as they are stored: fetched when it is done with the one before, converted (which
             // waits for them) when they are used
             uint32_t sc[kGroupsPer][4], zp[kGroupsPer][4];
+            const size_t tile0 = ((size_t)t.expert * x.n + n0) * groups_per_row;   // the offsets inside a tile fit 32 bits
+            const uint16_t* scale16 = reinterpret_cast<const uint16_t*>(x.scale) + tile0;
+            const uint32_t* scale32 = reinterpret_cast<const uint32_t*>(x.scale) + tile0;
+            uint32_t at0[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) at0[j] = (chan[j] - t.expert * x.n - n0) * groups_per_row;
             auto load_scales = [&](uint32_t kb) {
                 if constexpr (!GROUPED) return;
                 if (kb >= ns) return;
@@ -175,11 +186,17 @@ expert_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const FewParams p)
                 for (int q = 0; q < kGroupsPer; ++q) {
                     const uint32_t k = kb * (2 * CH) + q * (2 * CH / kGroupsPer);
                     if (k >= x.k) break;
+                    const uint32_t grp = k >> x.group_shift;
+                    if (half_scale) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const size_t at = (size_t)chan[j] * groups_per_row + (k >> x.group_shift);
-                        sc[q][j] = half_scale ? reinterpret_cast<const uint16_t*>(x.scale)[at] : reinterpret_cast<const uint32_t*>(x.scale)[at];
-                        if (has_zero) zp[q][j] = x.zero[at];
+                        for (int j = 0; j < 4; ++j) sc[q][j] = scale16[at0[j] + grp];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) sc[q][j] = scale32[at0[j] + grp];
+                    }
+                    if (has_zero) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) zp[q][j] = x.zero[tile0 + at0[j] + grp];
                     }
                 }
             };
@@ -191,14 +208,10 @@ expert_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const FewParams p)
                 for (int nt = 0; nt < MT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[m][nt][e] = 0.f;
-            uint32_t kb = (way - before) & (kWays - 1);
-            Ring r;
-            r.set(before + kb, kStages);
-            load_scales(kb);
-            for (; kb < ns; kb += kWays) {
-                ok = ok && warp_wait(full(r.i), r.phase, abort_flag);
-                if (!ok) { give_up(73, i, kb); break; }
-                const uint32_t stage = base + kOffStage + r.i * kStageAll;
+            // One stage: NT tiles of 8 rows.
+            auto work = [&](auto tiles_of_rows, uint32_t kb, uint32_t at) {
+                constexpr int NT = decltype(tiles_of_rows)::value;
+                const uint32_t stage = base + kOffStage + at * kStageAll;
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {   // 64 bytes of k
                     if (c == 1 && kb * (2 * CH) + CH >= x.k) break;
@@ -214,8 +227,8 @@ expert_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const FewParams p)
                             w[j][0] = v.x; w[j][1] = v.y; w[j][2] = v.z; w[j][3] = v.w;
                         }
                     }
-                    float part[2][MT][4];
-                    uint4 b[MT];
+                    float part[2][NT][4];
+                    uint4 b[NT];
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {   // words of the 16 bytes
                         const int grp = !GROUPED ? 0 : HALF ? 2 * c + q / 2 : c;
@@ -225,7 +238,7 @@ expert_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const FewParams p)
                         }
                         if (BITS == 4 || q % 2 == 0) {
 #pragma unroll
-                            for (int nt = 0; nt < MT; ++nt) b[nt] = lds128(act + act_off[BITS == 4 ? q : q / 2] + nt * (8 * kRowBytes / 2));
+                            for (int nt = 0; nt < NT; ++nt) b[nt] = lds128(act + act_off[BITS == 4 ? q : q / 2] + nt * (8 * kRowBytes / 2));
                         }
 #pragma unroll
                         for (int m = 0; m < 2; ++m) {
@@ -235,12 +248,17 @@ expert_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const FewParams p)
                                 s8x4_to_bf16(w[2 * m][q], flip, sel0, sel1, kMulByte, aa, fa[0], fa[1]);
                                 s8x4_to_bf16(w[2 * m + 1][q], flip, sel0, sel1, kMulByte, ab, fb[0], fb[1]);
                             } else {
-                                s4x8_to_bf16(w[2 * m][q], flip, nib, nib.mul[0], nib.mul[1], aa, fa);
-                                s4x8_to_bf16(w[2 * m + 1][q], flip, nib, nib.mul[0], nib.mul[1], ab, fb);
+                                if constexpr (PACKED) {
+                                    s4x8_to_bf16_strided(w[2 * m][q], flip, aa, fa);
+                                    s4x8_to_bf16_strided(w[2 * m + 1][q], flip, ab, fb);
+                                } else {
+                                    s4x8_to_bf16(w[2 * m][q], flip, nib, nib.mul[0], nib.mul[1], aa, fa);
+                                    s4x8_to_bf16(w[2 * m + 1][q], flip, nib, nib.mul[0], nib.mul[1], ab, fb);
+                                }
                             }
                             const bool first = GROUPED && (q == 0 || (HALF && q == 2)), last = GROUPED && (q == 3 || (HALF && q == 1));
 #pragma unroll
-                            for (int nt = 0; nt < MT; ++nt) {
+                            for (int nt = 0; nt < NT; ++nt) {
                                 if (BITS == 8) {
                                     const uint32_t b0 = q % 2 == 0 ? b[nt].x : b[nt].z, b1 = q % 2 == 0 ? b[nt].y : b[nt].w;
                                     if (!GROUPED) mma_bf16(acc[m][nt], fa[0], fb[0], fa[1], fb[1], b0, b1);
@@ -261,6 +279,15 @@ expert_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const FewParams p)
                         }
                     }
                 }
+            };
+            uint32_t kb = (way - before) & (kWays - 1);
+            Ring r;
+            r.set(before + kb, kStages);
+            load_scales(kb);
+            for (; kb < ns; kb += kWays) {
+                ok = ok && warp_wait(full(r.i), r.phase, abort_flag);
+                if (!ok) { give_up(73, i, kb); break; }
+                if (MT > 1 && two) work(Tiles<MT>(), kb, r.i); else work(Tiles<1>(), kb, r.i);
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(empty(r.i));
                 load_scales(kb + kWays);
@@ -306,9 +333,9 @@ expert_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const FewParams p)
     }
 }
 
-template <int BITS, int MT, bool GROUPED, bool HALF>
+template <int BITS, int MT, bool GROUPED, bool HALF, bool PACKED = false>
 int launch_cfg(const CUtensorMap& tw, const FewParams& q, DeviceCtx* ctx, cudaStream_t s) {
-    auto kern = expert_few_kernel<BITS, MT, GROUPED, HALF>;
+    auto kern = expert_few_kernel<BITS, MT, GROUPED, HALF, PACKED>;
     FewParams p = q;
     p.off_sums = kOffStage + kStages * (2 * kHalfBytes + 8 * MT * (BITS == 8 ? 256 : 512));
     p.off_table = p.off_sums + kWays * 8 * MT * kSumPitch * sizeof(float);
@@ -316,7 +343,11 @@ int launch_cfg(const CUtensorMap& tw, const FewParams& q, DeviceCtx* ctx, cudaSt
     if (bytes > 232448) return AFB_ERR_UNSUPPORTED;   // the caller has seen to it
     static DeviceOnce attr_set;
     if (!attr_set.done(ctx->device)) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+        cudaFuncAttributes attr;
+        cudaError_t e = cudaFuncGetAttributes(&attr, kern);
+        if (e != cudaSuccess) return cuda_fail(e);
+        if ((uint32_t)(attr.numRegs * kFewThreads) < kRegsAll) return AFB_ERR_UNSUPPORTED;   // the shares come out of what the block is launched with
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
         if (e != cudaSuccess) return cuda_fail(e);
         attr_set.mark(ctx->device);
     }
@@ -332,6 +363,10 @@ int launch_cfg(const CUtensorMap& tw, const FewParams& q, DeviceCtx* ctx, cudaSt
 template <int MT>
 int launch_rows(const CUtensorMap& tw, const FewParams& p, uint32_t bits, uint32_t group, DeviceCtx* ctx, cudaStream_t s) {
     if (bits == 8) return group ? launch_cfg<8, MT, true, false>(tw, p, ctx, s) : launch_cfg<8, MT, false, false>(tw, p, ctx, s);
+    if (p.x.packed) {
+        if (group == 64) return launch_cfg<4, MT, true, true, true>(tw, p, ctx, s);
+        return group ? launch_cfg<4, MT, true, false, true>(tw, p, ctx, s) : launch_cfg<4, MT, false, false, true>(tw, p, ctx, s);
+    }
     if (group == 64) return launch_cfg<4, MT, true, true>(tw, p, ctx, s);
     return group ? launch_cfg<4, MT, true, false>(tw, p, ctx, s) : launch_cfg<4, MT, false, false>(tw, p, ctx, s);
 }
@@ -390,7 +425,7 @@ extern "C" int afb_expert_gemm_launch(const afb_expert_gemm_args* x, void* strea
     p.enc = a.b_encoding; p.scale_dtype = a.scale_dtype; p.packed = a.b_layout == AFB_LAYOUT_COL_PACKED ? 1u : 0u;
     for (uint32_t g = a.group_size; g > 1; g >>= 1) ++p.group_shift;
     p.gated = x->gated; p.silu = x->activation == AFB_ACT_SILU ? 1u : 0u;
-    const bool many = a.variant == AFB_VARIANT_PREFILL || (a.variant == AFB_VARIANT_AUTO && (uint64_t)a.m > 24ull * x->experts);
+    const bool many = a.variant == AFB_VARIANT_PREFILL || (a.variant == AFB_VARIANT_AUTO && (uint64_t)a.m > (a.b_bits == 8 ? 10ull : 16ull) * x->experts);
     if (many && x->a_rows) {
         bool done = false;
         const int rc = launch_expert_many(p, a.b_bits, a.group_size, ctx, (cudaStream_t)stream, &done);

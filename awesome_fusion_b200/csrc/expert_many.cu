@@ -8,8 +8,8 @@
 //   warp 0        TMA: raw weight blocks, 128 channels x 128 bytes, 128-byte swizzle
 //   warp 2        rank 0: tcgen05.mma 256 x height x 16;  rank 1: reports to rank 0 that its half of a step is complete
 //   warps 4-11    epilogue, two per lane quarter: accumulator -> registers -> (accumulator free) -> shared memory -> C
-//   warps 12-19   converters: two groups of four warps; group g takes every second step of k (KS = 128 or 64 wide)
-//   warps 20-23   the rows of A: 16-byte copies to shared memory, written in the 128-byte swizzle.  (A TMA gather of four rows takes 65 cycles of
+//   then          converters: CG groups of four warps; group g takes every CG-th step of k (KS = 128 or 64 wide)
+//   last four     the rows of A: 16-byte copies to shared memory, written in the 128-byte swizzle.  (A TMA gather of four rows takes 65 cycles of
 //                 the issuing warp, which has to make every lane's row numbers uniform first: 4200 cycles per step of 256 rows.)
 //
 // The sum over all of K stays in the accumulator.  Scales per channel multiply it in the end.  Scales per group go into the weights, and there bf16 has no
@@ -29,11 +29,15 @@
 namespace afb {
 namespace {
 
-constexpr int kConvGroups = 2;
-constexpr int kFirstEpi = 4, kEpiWarps = 8, kFirstConv = kFirstEpi + kEpiWarps, kFirstLoad = kFirstConv + 4 * kConvGroups, kLoadWarps = 4;
-constexpr int kManyThreads = 32 * (kFirstLoad + kLoadWarps);   // 768: launched with 80 registers a thread
-constexpr uint32_t kRegsCtrl = 40, kRegsEpi = 136, kRegsConv = 64, kRegsLoad = 40;
-static_assert(128 * kRegsCtrl + 32 * kEpiWarps * kRegsEpi + 128 * kConvGroups * kRegsConv + 32 * kLoadWarps * kRegsLoad <= 80 * kManyThreads, "shares of the registers");
+constexpr int kFirstEpi = 4, kEpiWarps = 8, kFirstConv = kFirstEpi + kEpiWarps, kLoadWarps = 4;
+// CG groups of converters: four where strips are low and a group's chain (wait, load, unpack, tcgen05.st, arrive: 1800 cycles) is what a step waits for, two where
+// they are high and more warps only get in each other's way (1024 rows on 64 experts of 2048 x 4096 int4: 141 us with four, 153 with two; 16384 rows: 340, 320).
+__host__ __device__ constexpr int many_threads(int cg) { return 32 * (kFirstConv + 4 * cg + kLoadWarps); }        // 1024 or 768: launched with 64 or 80 registers a thread
+constexpr uint32_t kRegsCtrl = 40, kRegsLoad = 40;
+__host__ __device__ constexpr uint32_t regs_epi(int cg) { return cg == 4 ? 104 : 136; }
+__host__ __device__ constexpr uint32_t regs_conv(int cg) { return cg == 4 ? 56 : 64; }
+__host__ __device__ constexpr uint32_t regs_all(int cg) { return 128 * kRegsCtrl + 32 * kEpiWarps * regs_epi(cg) + 128 * cg * regs_conv(cg) + 32 * kLoadWarps * kRegsLoad; }
+static_assert(regs_all(2) <= 80u * many_threads(2) && regs_all(4) <= 64u * many_threads(4), "shares of the registers");
 constexpr int kMaxRaw = 12, kMaxSlots = 8, kMaxAcc = 2;
 __host__ __device__ constexpr uint32_t slots(int ks) { return ks == 128 ? 4 : 6; }   // steps under way, in 256 columns at most
 constexpr uint32_t kTmemCols = 512;
@@ -147,12 +151,13 @@ __global__ void __launch_bounds__(kPrepareThreads) expert_prepare_kernel(const P
 
 struct Strip : ExpertStrip { uint32_t n0; };   // n0: of this CTA's 128 channels
 
-template <int BITS, bool GROUPED, int KS>
-__global__ void __launch_bounds__(kManyThreads, 1)
+template <int BITS, bool GROUPED, int KS, int CG>
+__global__ void __launch_bounds__(many_threads(CG), 1)
 expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams p) {
     constexpr uint32_t SPB = (BITS == 8 ? 128 : 256) / KS;   // steps per raw block
     constexpr uint32_t kSlotCols = KS / 2;                   // TMEM columns of a step's weights
     constexpr uint32_t kSlots = slots(KS);
+    constexpr int kConvGroups = CG, kFirstLoad = kFirstConv + 4 * CG;
     extern __shared__ uint8_t smem_raw_base[];
     const uint32_t smem_base = (ptx::smem_u32(smem_raw_base) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw_base + (smem_base - ptx::smem_u32(smem_raw_base));
@@ -273,7 +278,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
         }
     } else if (warp >= kFirstConv && warp < kFirstLoad) {
         // ======================= converters =======================
-        ptx::regs_down<kRegsConv>();
+        ptx::regs_down<regs_conv(CG)>();
         const uint32_t g = (uint32_t)(warp - kFirstConv) >> 2, quarter = (uint32_t)warp & 3u;
         const uint32_t ch = quarter * 32 + lane;
         const uint32_t flip = BITS == 8 ? flip8(p.x.enc) : flip4(p.x.enc);
@@ -425,7 +430,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
             if (issued & (1u << s)) (void)warp_wait(step_empty(s), (parity >> s) & 1u, abort_flag);
     } else {
         // ======================= epilogue =======================
-        ptx::regs_up<kRegsEpi>();
+        ptx::regs_up<regs_epi(CG)>();
         const uint32_t quarter = (uint32_t)warp & 3u, half = (uint32_t)(warp - kFirstEpi) >> 2, ch = quarter * 32 + lane;
         constexpr int kPacks = 8;   // of 16 columns: this warp's half of a strip
         const bool odd = lane & 1, gated = p.x.gated != 0, act = p.x.silu != 0;
@@ -556,17 +561,21 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
     }
 }
 
-template <int BITS, bool GROUPED, int KS>
-int launch_cfg(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uint32_t smem, DeviceCtx* ctx, cudaStream_t s) {
-    auto kern = expert_many_kernel<BITS, GROUPED, KS>;
+template <int BITS, bool GROUPED, int KS, int CG>
+int launch_groups(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uint32_t smem, DeviceCtx* ctx, cudaStream_t s) {
+    auto kern = expert_many_kernel<BITS, GROUPED, KS, CG>;
     static DeviceOnce attr_set;  // per template instance
     if (!attr_set.done(ctx->device)) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+        cudaFuncAttributes attr;
+        cudaError_t e = cudaFuncGetAttributes(&attr, kern);
+        if (e != cudaSuccess) return cuda_fail(e);
+        if ((uint32_t)(attr.numRegs * many_threads(CG)) < regs_all(CG)) return AFB_ERR_UNSUPPORTED;   // the shares come out of what the block is launched with
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
         if (e != cudaSuccess) return cuda_fail(e);
         attr_set.mark(ctx->device);
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(kManyThreads); cfg.stream = s; cfg.dynamicSmemBytes = smem;
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(many_threads(CG)); cfg.stream = s; cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
@@ -574,6 +583,11 @@ int launch_cfg(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uint32
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, p);
     count_launch();
     return e == cudaSuccess ? AFB_OK : cuda_fail(e);
+}
+
+template <int BITS, bool GROUPED, int KS>
+int launch_cfg(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uint32_t smem, DeviceCtx* ctx, cudaStream_t s) {
+    return p.x.tile_rows <= 128 ? launch_groups<BITS, GROUPED, KS, 4>(tw, p, grid, smem, ctx, s) : launch_groups<BITS, GROUPED, KS, 2>(tw, p, grid, smem, ctx, s);
 }
 
 }  // namespace
@@ -593,7 +607,7 @@ int launch_expert_many(const ExpertParams& q, uint32_t bits, uint32_t group, Dev
     p.raw_stages = (232448 - 1024 - p.off_raw - act_bytes) / kRawBytes;
     if (p.raw_stages > (uint32_t)kMaxRaw) p.raw_stages = kMaxRaw;
     // the parity waits of the converters: see stream.cu
-    const uint32_t per_block = p.steps % spb == 0 ? spb : 1;
+    const uint32_t per_block = p.steps % spb == 0 ? spb : 1, kConvGroups = p.x.tile_rows <= 128 ? 4 : 2;
     p.slot_first = p.raw_stages * per_block >= kConvGroups + kSlots + per_block - 1 ? 0u : 1u;
     if (p.raw_stages * per_block < kSlots + per_block - 1) return AFB_ERR_UNSUPPORTED;   // not with any size that this function takes
     p.c_vec = q.ldc % 8 == 0 && (uintptr_t)q.c % 16 == 0 && q.n_out % 8 == 0;
