@@ -36,6 +36,7 @@ struct FewParams {
     ExpertParams x;
     uint32_t stages_per_tile;   // along K
     uint32_t off_sums, off_table;
+    uint32_t c_vec;             // four results of a row (gated: two) in one store
     int32_t* status;
 };
 
@@ -51,6 +52,11 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src
 // Arrives on `bar` when this thread's copies so far are complete.
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+// The unpack's addend for a zero-point byte: -(the byte as an unsigned weight) * 2^-6, by the unpack's own multiply-add.
+template <int BITS> __device__ __forceinline__ uint32_t zero_addend(uint32_t zbyte, uint32_t flip) {
+    const uint32_t u = (zbyte ^ flip) & (BITS == 8 ? 0xffu : 0xfu);
+    return bf16x2_fma(u * 0x00010001u, kMulByte | 0x80008000u, 0u);
 }
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
     uint2 v;
@@ -166,10 +172,9 @@ expert_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const FewParams p)
             uint32_t chan[4];      // rows of B of this lane's channels: 8 apart
 #pragma unroll
             for (int j = 0; j < 4; ++j) chan[j] = t.expert * x.n + min(n0 + cg * 32 + j * 8 + g, x.n - 1);
-            auto zero_add = [&](size_t at) { return unpack_add(BITS, BITS == 8 ? decode_zero8(x.zero[at], x.enc) : decode_zero4(x.zero[at], x.enc)); };
             uint32_t add[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) add[j] = !GROUPED && has_zero ? zero_add(chan[j]) : unpack_add(BITS, 0);
+            for (int j = 0; j < 4; ++j) add[j] = !GROUPED && has_zero ? zero_addend<BITS>(x.zero[chan[j]], flip) : unpack_add(BITS, 0);
             // scales and zero-points of this warp's next stage, as they are stored: fetched when it is done with the one before, converted (which
             // waits for them) when they are used
             uint32_t sc[kGroupsPer][4], zp[kGroupsPer][4];
@@ -234,7 +239,7 @@ expert_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const FewParams p)
                         const int grp = !GROUPED ? 0 : HALF ? 2 * c + q / 2 : c;
                         if (GROUPED && has_zero && (q == 0 || (HALF && q == 2))) {
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) add[j] = unpack_add(BITS, BITS == 8 ? decode_zero8(zp[grp][j], x.enc) : decode_zero4(zp[grp][j], x.enc));
+                            for (int j = 0; j < 4; ++j) add[j] = zero_addend<BITS>(zp[grp][j], flip);
                         }
                         if (BITS == 4 || q % 2 == 0) {
 #pragma unroll
@@ -316,16 +321,31 @@ expert_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const FewParams p)
                     if (GROUPED) f[e] *= kUnpackInverse;
                     else f[e] = nn + e < x.n ? unscaled(f[e], load_scale(x.scale, (size_t)t.expert * x.n + nn + e, x.scale_dtype)) : 0.f;
                 }
-                if (x.gated) {
-                    uint16_t* dst = x.c + (size_t)(t.row0 + row) * x.ldc + nn / 2;
+                const int n_here = x.gated ? 2 : 4;
+                uint32_t o[2];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        if (nn + 2 * e < x.n) dst[e] = __bfloat16_as_ushort(__float2bfloat16_rn((x.silu ? silu(f[2 * e]) : f[2 * e]) * f[2 * e + 1]));
+                for (int e = 0; e < 2; ++e) {
+                    const float lo = x.silu ? silu(f[2 * e]) : f[2 * e], hi = f[2 * e + 1];
+                    if (x.gated) {
+                        f[e] = lo * hi;   // f[1] has been read
+                    } else {
+                        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, x.silu ? silu(hi) : hi);
+                        o[e] = *reinterpret_cast<const uint32_t*>(&v);
+                    }
+                }
+                if (x.gated) {
+                    const __nv_bfloat162 v = __floats2bfloat162_rn(f[0], f[1]);
+                    o[0] = *reinterpret_cast<const uint32_t*>(&v);
+                }
+                const uint32_t col = x.gated ? nn / 2 : nn;
+                uint16_t* dst = x.c + (size_t)(t.row0 + row) * x.ldc + col;
+                if (p.c_vec && col + n_here <= x.n_out) {
+                    if (x.gated) *reinterpret_cast<uint32_t*>(dst) = o[0];
+                    else *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
                 } else {
-                    uint16_t* dst = x.c + (size_t)(t.row0 + row) * x.ldc + nn;
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (nn + e < x.n) dst[e] = __bfloat16_as_ushort(__float2bfloat16_rn(x.silu ? silu(f[e]) : f[e]));
+                        if (e < n_here && col + e < x.n_out) dst[e] = (uint16_t)(o[e / 2] >> (e % 2 * 16));
                 }
             }
             asm volatile("bar.sync 1, %0;" ::"n"(32 * kFewWarps) : "memory");
@@ -378,6 +398,7 @@ int launch_expert_few(const ExpertParams& q, uint32_t bits, uint32_t group, Devi
     p.x = q;
     p.x.n_blocks = (q.n + kCh - 1) / kCh;
     p.stages_per_tile = (uint32_t)(((uint64_t)q.k * bits / 8 + 127) / 128);
+    p.c_vec = q.ldc % 4 == 0 && (uintptr_t)q.c % 8 == 0;
     p.status = ctx->status;
     // tiles of 8 rows where few experts have more; of int4 also where the table of many experts leaves no room for the rows of 16
     const bool small = (uint64_t)q.m <= 3ull * q.experts || (bits == 4 && q.experts > 128);
@@ -408,7 +429,7 @@ extern "C" int afb_expert_gemm_launch(const afb_expert_gemm_args* x, void* strea
     if (a.k % (a.b_bits == 8 ? 64u : 128u) || a.lda % 8 || ((uint64_t)a.ldb * a.b_bits / 8) % 16) return AFB_ERR_UNSUPPORTED;
     if ((uintptr_t)a.ptr_a % 16 || (uintptr_t)a.ptr_b % 16) return AFB_ERR_UNSUPPORTED;
     if (a.group_size && (a.group_size < 64 || (a.group_size & (a.group_size - 1)))) return AFB_ERR_UNSUPPORTED;
-    if (a.m >> 31 || x->a_rows >> 31 || ((uint64_t)x->experts * a.n) >> 31) return AFB_ERR_TOO_LARGE;
+    if (a.k >> 24 || a.m >> 31 || x->a_rows >> 31 || ((uint64_t)x->experts * a.n) >> 31) return AFB_ERR_TOO_LARGE;
     DeviceCtx* ctx = current_ctx();
     if (!ctx) return AFB_ERR_NOT_INIT;
     if (a.m == 0) return AFB_OK;

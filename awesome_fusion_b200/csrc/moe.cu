@@ -13,10 +13,10 @@
 namespace afb {
 namespace {
 
-constexpr int kRouteThreads = 512, kRouteWarps = kRouteThreads / 32;
+constexpr int kOneThreads = 512, kOneWarps = kOneThreads / 32, kRouteThreads = 1024, kRouteWarps = kRouteThreads / 32;
 constexpr uint32_t kOneBlockPairs = 512;   // up to here one CTA: its ranks are counted pair against pair
 constexpr uint32_t kMaxBlocks = 256;       // of the two-kernel form: every block reads all blocks' counts
-constexpr uint32_t kMinBlockTokens = 16;   // one per warp
+constexpr uint32_t kMinBlockTokens = 32;   // one per warp
 
 struct RouteParams {
     const void* logits;
@@ -101,13 +101,13 @@ __device__ __forceinline__ void scan_experts(const int32_t* count, int32_t* star
 }
 
 template <int NV>
-__global__ void __launch_bounds__(kRouteThreads) route_one_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(kOneThreads) route_one_kernel(const RouteParams p) {
     __shared__ int32_t s_id[kOneBlockPairs];
     __shared__ int32_t s_count[AFB_MOE_MAX_EXPERTS], s_start[AFB_MOE_MAX_EXPERTS + 1];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, pairs = p.tokens * p.top_k;
-    for (uint32_t e = tid; e < p.experts; e += kRouteThreads) s_count[e] = 0;
+    for (uint32_t e = tid; e < p.experts; e += kOneThreads) s_count[e] = 0;
     __syncthreads();
-    for (uint32_t t = warp; t < p.tokens; t += kRouteWarps) {
+    for (uint32_t t = warp; t < p.tokens; t += kOneWarps) {
         int32_t id; float w;
         pick_token<NV>(p, t, lane, id, w);
         if (lane < p.top_k) {
@@ -121,9 +121,9 @@ __global__ void __launch_bounds__(kRouteThreads) route_one_kernel(const RoutePar
     __syncthreads();
     if (warp == 0) scan_experts(s_count, s_start, p.experts, lane);
     __syncthreads();
-    for (uint32_t e = tid; e <= p.experts; e += kRouteThreads) p.offsets[e] = s_start[e];
+    for (uint32_t e = tid; e <= p.experts; e += kOneThreads) p.offsets[e] = s_start[e];
     const uint32_t rows = (uint32_t)s_start[p.experts];
-    for (uint32_t i = tid; i < pairs; i += kRouteThreads) {
+    for (uint32_t i = tid; i < pairs; i += kOneThreads) {
         const int32_t id = s_id[i];
         int32_t row = -1;
         if (id >= 0) {
@@ -169,36 +169,41 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteP
     for (uint32_t i = tid; i < kRouteWarps * p.experts; i += kRouteThreads) s_next[i] = 0;
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    // this block's pairs in runs, one per warp; the first 32 of a run are fetched once, ahead of the counts
+    const size_t i0 = (size_t)blockIdx.x * p.block_tokens * p.top_k;
+    const uint32_t mine = (uint32_t)(min(p.tokens, (blockIdx.x + 1) * p.block_tokens) - blockIdx.x * p.block_tokens) * p.top_k;
+    const uint32_t run = (mine + kRouteWarps - 1) / kRouteWarps, r0 = min(mine, warp * run), r1 = min(mine, r0 + run);
+    auto id_at = [&](uint32_t r) { return r < r1 ? __ldcg(p.ids + i0 + r) : -1; };
+    const int32_t first_id = id_at(r0 + lane);
     // counts of all blocks: the threads of one expert (or of one of its stretches) take every `parts`-th block
     const uint32_t parts = p.experts >= kRouteThreads ? 1u : kRouteThreads / p.experts;
     for (uint32_t e = tid % min(p.experts, (uint32_t)kRouteThreads); e < p.experts; e += kRouteThreads) {
         const uint32_t part = p.experts >= kRouteThreads ? 0u : tid / p.experts;
         if (part >= parts) break;
         int32_t all = 0, before = 0;
-#pragma unroll 8
+#pragma unroll 16
         for (uint32_t b = part; b < p.blocks; b += parts) {
             const int32_t c = __ldcg(p.counts + (size_t)b * p.experts + e);
             all += c;
-            if (b < blockIdx.x) before += c;
+            before += b < blockIdx.x ? c : 0;
         }
         atomicAdd(&s_all[e], all);
         atomicAdd(&s_before[e], before);
     }
-    // this block's pairs in runs, one per warp
-    const size_t i0 = (size_t)blockIdx.x * p.block_tokens * p.top_k;
-    const uint32_t mine = (uint32_t)(min(p.tokens, (blockIdx.x + 1) * p.block_tokens) - blockIdx.x * p.block_tokens) * p.top_k;
-    const uint32_t run = (mine + kRouteWarps - 1) / kRouteWarps, r0 = min(mine, warp * run), r1 = min(mine, r0 + run);
     int32_t* next = s_next + warp * p.experts;
     for (uint32_t r = r0 + lane; r < r1; r += 32) {
-        const int32_t id = __ldcg(p.ids + i0 + r);
+        const int32_t id = r < r0 + 32 ? first_id : id_at(r);
         if (id >= 0) atomicAdd(&next[id], 1);
     }
     __syncthreads();
     if (warp == 0) scan_experts(s_all, s_start, p.experts, lane);
     __syncthreads();
     for (uint32_t e = tid; e < p.experts; e += kRouteThreads) {
-        int32_t row = s_start[e] + s_before[e];
-        for (uint32_t w = 0; w < (uint32_t)kRouteWarps; ++w) { const int32_t c = s_next[w * p.experts + e]; s_next[w * p.experts + e] = row; row += c; }
+        int32_t row = s_start[e] + s_before[e], c[kRouteWarps];
+#pragma unroll
+        for (int w = 0; w < kRouteWarps; ++w) c[w] = s_next[w * p.experts + e];
+#pragma unroll
+        for (int w = 0; w < kRouteWarps; ++w) { s_next[w * p.experts + e] = row; row += c[w]; }
     }
     if (blockIdx.x == 0)
         for (uint32_t e = tid; e <= p.experts; e += kRouteThreads) p.offsets[e] = s_start[e];
@@ -206,7 +211,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteP
     const uint32_t rows = (uint32_t)s_start[p.experts];
     for (uint32_t r = r0; r < r1; r += 32) {
         const bool there = r + lane < r1;
-        const int32_t id = there ? __ldcg(p.ids + i0 + r + lane) : -1;
+        const int32_t id = r == r0 ? first_id : id_at(r + lane);
         const uint32_t same = __match_any_sync(0xffffffffu, id), below = same & ((1u << lane) - 1u);
         int32_t row = -1;
         if (id >= 0) row = next[id] + __popc(below);
@@ -235,7 +240,7 @@ uint32_t route_block_tokens(uint32_t tokens) {
 template <int NV>
 int launch_route(const RouteParams& p, DeviceCtx* ctx, cudaStream_t s) {
     if ((uint64_t)p.tokens * p.top_k <= kOneBlockPairs) {
-        route_one_kernel<NV><<<1, kRouteThreads, 0, s>>>(p);
+        route_one_kernel<NV><<<1, kOneThreads, 0, s>>>(p);
         count_launch();
         const cudaError_t e = cudaGetLastError();
         return e == cudaSuccess ? AFB_OK : cuda_fail(e);

@@ -246,13 +246,17 @@ int afb_moe_route_launch(const afb_moe_route_args* args, void* stream);
  *              [experts, n, k / group_size]
  *     b_layout AFB_LAYOUT_COL or AFB_LAYOUT_COL_PACKED (afb_prepack / afb_prepack_gated of all experts at once: a matrix of experts * n rows)
  *     group_size 0, or a power of two of at least 64;  k a multiple of 64 (int8) or 128 (int4);  lda a multiple of 8, A 16-byte aligned, rows
- *              of B and ptr_b 16-byte aligned; any n and ldc.  Otherwise AFB_ERR_UNSUPPORTED
+ *              of B and ptr_b 16-byte aligned; any n and ldc.  Otherwise AFB_ERR_UNSUPPORTED.  k < 2^24, m, a_rows and experts * n < 2^31
  *     variant  AFB_VARIANT_AUTO, AFB_VARIANT_DECODE (form for few rows per expert: weights streamed through registers) or
  *              AFB_VARIANT_PREFILL (form for many: tcgen05);  flags 0.
  *     C[r,:] = f(A[row(r),:] x dequant(B[e])^T)   for offsets[e] <= r < offsets[e + 1]
  *     row(r) = ptr_row_pair[r] / top_k (the first product: A holds the tokens), or r where ptr_row_pair is NULL (the second one)
  *     f: nothing, the activation, or gated: act(v[2i]) * v[2i + 1] into n / 2 columns
- * in fp32 from the fp32 sums; group scales multiply the fp32 sum of each group in both forms; rounded to bf16 once.
+ * in fp32 from the fp32 sums, rounded to bf16 once.  Group scales multiply the fp32 sum of each group in the form for few rows.  In the form for many they
+ * multiply the weights, in fp16: the product is exact for int4 without zero-points and bf16 scales, else off by 2^-11 of itself at most (2^-10 for fp32
+ * scales); rows of A and the scales of a channel are given a power of two for that, and of the row's values what is below 2^-28 of the largest (of the
+ * scales 2^-20) keeps fewer bits.  This form converts the rows of A into a workspace of the stream or captured graph first, as the streaming form
+ * has one; where there is none to be had the other form runs.
  * The offsets are read on the GPU.  They must not fall; values outside 0 .. m are taken as the nearer end.  A row(r) outside
  * 0 .. a_rows - 1 reads as a row of zeros. */
 typedef struct afb_expert_gemm_args {

@@ -54,7 +54,7 @@ def test_route_refuses(lib, changes):
 def test_route_sizes(lib):
     assert _route(lib, tokens=1 << 30) == E_LARGE
     assert lib.moe_route_workspace(1, 64) == 0 and lib.moe_route_workspace(0, 64) == 0
-    assert lib.moe_route_workspace(4096, 128) == 256 * 128 * 4
+    assert lib.moe_route_workspace(4096, 128) == 128 * 128 * 4
     assert lib.lib.afb_moe_route_workspace(1, 0, ctypes.byref(ctypes.c_uint64())) == E_BAD
     assert lib.lib.afb_moe_route_workspace(1, 1025, ctypes.byref(ctypes.c_uint64())) == E_BAD
     assert lib.lib.afb_moe_route_workspace(1, 8, None) == E_BAD
@@ -92,6 +92,7 @@ def test_expert_gemm_sizes(lib):
     assert _expert(lib, dict(m=1 << 31)) == E_LARGE
     assert _expert(lib, {}, a_rows=1 << 31) == E_LARGE
     assert _expert(lib, dict(n=1 << 28, ldc=1 << 28)) == E_LARGE
+    assert _expert(lib, dict(k=1 << 24, lda=1 << 24, ldb=1 << 24)) == E_LARGE
 
 
 def _combine(lib, **changes):
@@ -205,7 +206,9 @@ class Experts:
 
 
 def check(got, want, off):
-    bad = (got.double() - want).abs() > off
+    rounded = want.to(got.dtype)
+    over = rounded.isinf()   # above the largest bf16: infinity is the result
+    bad = torch.where(over, got != rounded, (got.double() - want).abs() > off)
     assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} too far off, first at {bad.nonzero()[0].tolist()}: {got[bad][0]} for {want[bad][0]} +- {off[bad][0]}"
 
 
@@ -364,6 +367,80 @@ def test_expert_gemm_takes_bad_plans(afb, variant):
     x.run(afb, a, offsets, row_pair, 1, variant=variant, rows=8, out=guard[6:14])
     assert torch.equal(guard[6:14], got) and (guard[:6] == 777).all() and (guard[14:] == 777).all()
     assert afb.read_status()[0] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", FORMS)
+@pytest.mark.parametrize("fmt", [dict(bits=4, group=128), dict(bits=8, group=64, zero=True), dict(bits=8), dict(bits=4, zero=True, group=64, packed=True)],
+                         ids=lambda f: "-".join(f"{k}{v}" for k, v in f.items()))
+def test_expert_gemm_ranges(afb, variant, fmt):
+    """Rows of A from 2^-90 to 2^90, with one value far above the others, of zeros; channels whose scales differ by powers of two, are negative or zero."""
+    x = Experts(3, 140, 512, seed=15, **fmt)
+    counts = [40, 3, 50]
+    offsets, a = offsets_of(counts), activations(sum(counts), 512)
+    a = (a.float() * 2.0 ** torch.linspace(-90, 90, a.shape[0], device="cuda").round()[:, None]).bfloat16()
+    a[4] = 0
+    a[7, 100] = a[7, 100].abs().clamp(min=2.0 ** -80) * 2.0 ** 20
+    a[60, 3] = 2.0 ** 120
+    factor = 2.0 ** torch.randint(-7, 8, x.scale.shape, generator=torch.Generator().manual_seed(1)).cuda().float()
+    factor[:, ::9] *= -1
+    factor[:, 5] = 0
+    x.scale = (x.scale.float() * factor).to(x.scale.dtype)
+    x.w = x.w * (factor.double().repeat_interleave(x.group, 2) if x.group else factor.double()[..., None])
+    want, off = x.plain(a, offsets, variant=variant)
+    # what fp16 loses at the ends of its range: 2^-40 of the row's largest value, times the weights; a scale keeps all its bits (2^14 between them)
+    for e in range(3):
+        lo, hi = sum(counts[:e]), sum(counts[: e + 1])
+        off[lo:hi] += 2.0 ** -40 * a[lo:hi].double().abs().amax(1, keepdim=True) * x.w[e].abs().sum(1)
+    check(x.run(afb, a, offsets, variant=variant), want, off)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", FORMS)
+@pytest.mark.parametrize("bits, group", [(4, 128), (8, 0), (8, 64)])
+def test_expert_gemm_of_many_experts(afb, variant, bits, group):
+    """The table of 1000 experts, most of them without a row."""
+    x = Experts(1000, 24, 256, bits, group, seed=17)
+    rng = np.random.default_rng(3)
+    counts = np.where(rng.random(1000) < 0.1, rng.integers(1, 20, 1000), 0)
+    counts[[0, 999]] = 1, 300
+    offsets, a = offsets_of(counts), activations(int(counts.sum()), 256)
+    check(x.run(afb, a, offsets, variant=variant), *x.plain(a, offsets, variant=variant))
+
+
+@pytest.mark.gpu
+def test_expert_gemm_without_workspace(afb):
+    """cudaStreamPerThread names no stream to keep a workspace for: the form for few rows takes what would need one."""
+    x = Experts(2, 72, 256, 4, 128, seed=19)
+    offsets, a = offsets_of([90, 30]), activations(120, 256)
+    got = x.run(afb, a, offsets, variant=pkg.VARIANT_PREFILL, stream=2)
+    torch.cuda.synchronize()
+    assert torch.equal(got, x.run(afb, a, offsets, variant=pkg.VARIANT_DECODE))
+
+
+@pytest.mark.gpu
+def test_expert_gemm_in_two_graphs_at_once(afb):
+    """Two captured graphs, and the stream that they were captured on, at the same time: each has a workspace of its own."""
+    x = Experts(8, 264, 1024, 4, 128, seed=21)
+    counts = [100, 3, 260, 0, 40, 77, 1, 90]
+    offsets, rows = offsets_of(counts), sum(counts)
+    inputs = [activations(rows, 1024, seed=s) for s in range(3)]
+    want = [x.run(afb, a, offsets, variant=pkg.VARIANT_PREFILL) for a in inputs]
+    outs, graphs, stream = [torch.zeros_like(w) for w in want], [], torch.cuda.Stream()
+    for a, out in list(zip(inputs, outs))[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            x.run(afb, a, offsets, variant=pkg.VARIANT_PREFILL, out=out, stream=torch.cuda.current_stream().cuda_stream)
+        graphs.append(graph)
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for graph, side in zip(graphs, sides):
+            with torch.cuda.stream(side):
+                graph.replay()
+        x.run(afb, inputs[2], offsets, variant=pkg.VARIANT_PREFILL, out=outs[2], stream=stream.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(w, o) for w, o in zip(want, outs))
 
 
 @pytest.mark.gpu
