@@ -38,7 +38,7 @@ __host__ __device__ constexpr uint32_t regs_epi(int cg) { return cg == 4 ? 104 :
 __host__ __device__ constexpr uint32_t regs_conv(int cg) { return cg == 4 ? 56 : 64; }
 __host__ __device__ constexpr uint32_t regs_all(int cg) { return 128 * kRegsCtrl + 32 * kEpiWarps * regs_epi(cg) + 128 * cg * regs_conv(cg) + 32 * kLoadWarps * kRegsLoad; }
 static_assert(regs_all(2) <= 80u * many_threads(2) && regs_all(4) <= 64u * many_threads(4), "shares of the registers");
-constexpr int kMaxRaw = 12, kMaxSlots = 8, kMaxAcc = 2;
+constexpr int kMaxRaw = 12, kMaxSlots = 8, kMaxAcc = 4;
 __host__ __device__ constexpr uint32_t slots(int ks) { return ks == 128 ? 4 : 6; }   // steps under way, in 256 columns at most
 constexpr uint32_t kTmemCols = 512;
 constexpr int kBars = 2 * (kMaxRaw + kMaxSlots + kMaxAcc);
@@ -151,13 +151,15 @@ __global__ void __launch_bounds__(kPrepareThreads) expert_prepare_kernel(const P
 
 struct Strip : ExpertStrip { uint32_t n0; };   // n0: of this CTA's 128 channels
 
-template <int BITS, bool GROUPED, int KS, int CG>
+template <int BITS, bool GROUPED, int KS, int CG, bool LOW>
 __global__ void __launch_bounds__(many_threads(CG), 1)
 expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams p) {
     constexpr uint32_t SPB = (BITS == 8 ? 128 : 256) / KS;   // steps per raw block
     constexpr uint32_t kSlotCols = KS / 2;                   // TMEM columns of a step's weights
     constexpr uint32_t kSlots = slots(KS);
     constexpr int kConvGroups = CG, kFirstLoad = kFirstConv + 4 * CG;
+    constexpr uint32_t kIssuers = LOW ? 2 : 1;
+    static_assert(!LOW || (CG == 4 && kSlots % 2 == 0), "a slot's steps are one issuer's");
     extern __shared__ uint8_t smem_raw_base[];
     const uint32_t smem_base = (ptx::smem_u32(smem_raw_base) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw_base + (smem_base - ptx::smem_u32(smem_raw_base));
@@ -179,8 +181,8 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
 
     if (warp == 0 && lane == 0) {
         for (uint32_t s = 0; s < p.raw_stages; ++s) { ptx::mbar_init(raw_full(s), 1); ptx::mbar_init(raw_empty(s), 4 * SPB); }
-        for (uint32_t s = 0; s < kSlots; ++s) { ptx::mbar_init(step_full(s), 4 + kLoadWarps + (rank == 0 ? 1 : 0)); ptx::mbar_init(step_empty(s), 1); }
-        for (uint32_t s = 0; s < p.accs; ++s) { ptx::mbar_init(acc_full(s), 1); ptx::mbar_init(acc_empty(s), 2 * kEpiWarps); }
+        for (uint32_t s = 0; s < kSlots; ++s) { ptx::mbar_init(step_full(s), 4 + (LOW ? 1 : kLoadWarps) + (rank == 0 ? 1 : 0)); ptx::mbar_init(step_empty(s), 1); }
+        for (uint32_t s = 0; s < p.accs * kIssuers; ++s) { ptx::mbar_init(acc_full(s), 1); ptx::mbar_init(acc_empty(s), 2 * kEpiWarps); }
         *abort_flag = 0;
         ptx::fence_mbar_init();
         ptx::prefetch_tmap(&tmap_w);
@@ -238,31 +240,37 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
             }
             for (uint32_t s = 0; s < p.raw_stages; ++s)   // never leave with a bulk copy still writing this CTA's shared memory
                 if (issued & (1u << s)) ptx::mbar_wait(raw_full(s), (parity >> s) & 1u);
-        } else if (warp == 2 && rank == 0) {
-            // ======================= MMA issuer =======================
+        } else if (rank == 0 && (uint32_t)warp - 2 < kIssuers) {
+            // ======================= MMA issuer(s) =======================
+            const uint32_t who = (uint32_t)warp - 2;
             const uint64_t desc0 = ptx::umma_desc_kmajor_sw128(smem_base + off_act);
-            Ring rc{0, 0};
+            r.i = who;
+            Ring rc{0, 0};       // of the accumulator, or of this issuer's of a tile's two
+            uint32_t before = 0, g = who;   // steps of the tiles walked so far; this warp's next step, counted over all tiles
             bool ready = false;
             while (ok && next(x)) {
                 const uint32_t idesc = GROUPED ? ptx::umma_idesc_f16_f32(2 * kCh, x.height) : ptx::umma_idesc_bf16_f32(2 * kCh, x.height), slab_d = x.height * 64u >> 4;
-                const uint32_t td = tmem_base + rc.i * acc_cols, acc_done = acc_full(rc.i);
-                if (!warp_wait(acc_empty(rc.i), rc.phase ^ 1u, abort_flag)) { give_up(63, x.expert, 0); break; }
-                rc.step(1, p.accs);
-                for (uint32_t l = 0; l < ns; ++l) {
-                    if (!__all_sync(0xffffffffu, ready) && !warp_wait(step_full(r.i), r.phase, abort_flag)) { give_up(64, x.expert, l); ok = false; break; }
+                const uint32_t acc = LOW ? 2 * rc.i + who : rc.i, td = tmem_base + acc * acc_cols, acc_done = acc_full(acc), first = g;
+                if (g < before + ns) {   // of a tile of one step one of the two issuers has none
+                    if (!warp_wait(acc_empty(acc), rc.phase ^ 1u, abort_flag)) { give_up(63, x.expert, 0); break; }
+                }
+                for (; g < before + ns; g += kIssuers) {
+                    if (!__all_sync(0xffffffffu, ready) && !warp_wait(step_full(r.i), r.phase, abort_flag)) { give_up(64, x.expert, g); ok = false; break; }
                     ptx::tc_fence_after_sync();
                     const uint32_t ta = slot_base + r.i * kSlotCols, done = step_empty(r.i);
                     const uint64_t db = desc0 + r.i * (act_stride >> 4);
-                    r.step(1, kSlots);
+                    r.step(kIssuers, kSlots);
                     ready = ptx::mbar_test_wait(step_full(r.i), r.phase);   // of the next step: the answer is back when this one has been issued
                     if (ptx::elect_one()) {
 #pragma unroll
                         for (int j = 0; j < KS / 16; ++j)
-                            ptx::umma_bf16_ts_pair(td, ta + 8 * j, db + (uint32_t)(j / 4) * slab_d + 2u * (j % 4), idesc, l > 0 || j > 0 ? 1u : 0u);   // kind::f16: the types are the descriptor's
+                            ptx::umma_bf16_ts_pair(td, ta + 8 * j, db + (uint32_t)(j / 4) * slab_d + 2u * (j % 4), idesc, g > first || j > 0 ? 1u : 0u);   // kind::f16: the types are the descriptor's
                         ptx::umma_commit_pair(done);
-                        if (l + 1 == ns) ptx::umma_commit_pair(acc_done);
+                        if (g + kIssuers >= before + ns) ptx::umma_commit_pair(acc_done);
                     }
                 }
+                before += ns;
+                rc.step(1, p.accs);
             }
         } else if (warp == 2) {
             // ======================= rank 1: reports its half of each step =======================
@@ -378,69 +386,115 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
         }
     } else if (warp >= kFirstLoad) {
         // ======================= rows of A =======================
-        // A lane copies 16 bytes of rows 16 * i + 4 * (which loader) + lane / 8 of this CTA's half, per 64 k.
         ptx::regs_down<kRegsLoad>();
-        const uint32_t r8 = (uint32_t)(warp - kFirstLoad) * 4 + ((uint32_t)lane >> 3), piece = (uint32_t)lane & 7u;
-        const uint32_t at = smem_base + off_act + r8 * 128u + ((piece ^ (r8 & 7u)) << 4);   // 16 rows on: the same place in the swizzle
-        Ring r{0, 0}, rp{0, 0};       // of the step that comes next, of the oldest one that has not been reported
-        uint32_t pending = 0, issued = 0, parity = 0;
-        bool ok = true;
-        // The copies are this thread's writes; tcgen05.mma reads shared memory through the asynchronous proxy.
-        auto report = [&] {
-            ptx::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(step_full(rp.i));
-            rp.step(1, kSlots);
-            --pending;
-        };
-        while (ok && next(x)) {
-            const uint32_t act_rows = x.height / 2, slab_bytes = act_rows * 128u;   // act_rows: a multiple of 16
-            uint32_t src[8];
+        if constexpr (LOW) {
+            // Low strips: each of the four warps takes every fourth step and waits for its copies, so that their latency is spread over four steps.  A lane
+            // copies 16 bytes of rows 4 * i + lane / 8 of this CTA's half, per 64 k; lane l knows where row l comes from.
+            const uint32_t who = (uint32_t)(warp - kFirstLoad), r4 = (uint32_t)lane >> 3, piece = (uint32_t)lane & 7u;
+            const uint32_t even = smem_base + off_act + r4 * 128u + ((piece ^ r4) << 4), odd = smem_base + off_act + (4 + r4) * 128u + ((piece ^ (4 + r4)) << 4);
+            Ring r{who, 0};
+            uint32_t before = 0, g = who;   // g: this warp's next step, counted over all tiles
+            bool ok = true;
+            while (ok && next(x)) {
+                const uint32_t act_rows = x.height / 2, slab_bytes = act_rows * 128u, c = rank * act_rows + lane;   // act_rows: 16 or 32
+                const uint32_t src = (uint32_t)lane < act_rows && c < x.rows ? source_row(p.x, x.row0 + c) : 0xffffffffu;   // none: zeros
+                for (; g < before + ns; g += kLoadWarps) {
+                    if (!warp_wait(step_empty(r.i), r.phase ^ 1u, abort_flag)) { give_up(62, x.expert, g); ok = false; break; }
+                    const uint32_t to = r.i * act_stride;
+                    const uint16_t* from = p.x.a + (g - before) * KS + piece * 8u;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {   // rows behind the last one, and those that A does not have: zeros
-                const uint32_t r0 = 16u * i + r8, c = rank * act_rows + r0;
-                src[i] = r0 < act_rows && c < x.rows ? source_row(p.x, x.row0 + c) : 0xffffffffu;
-            }
-            for (uint32_t l = 0; l < ns; ++l) {
-                // a free slot: go on; otherwise first report all that is under way
-                if (!__all_sync(0xffffffffu, ptx::mbar_test_wait(step_empty(r.i), r.phase ^ 1u))) {
-                    if (pending) { cp_async_wait_all(); while (pending) report(); }
-                    if (!warp_wait(step_empty(r.i), r.phase ^ 1u, abort_flag)) { give_up(62, x.expert, l); ok = false; break; }
+                    for (int i = 0; i < 8; ++i) {
+                        if (4u * i >= act_rows) break;
+                        const uint32_t row = __shfl_sync(0xffffffffu, src, i * 4 + r4);
+                        const bool there = row < p.x.a_rows;
+                        const uint16_t* at = there ? from + (size_t)row * p.x.lda : p.x.a;
+#pragma unroll
+                        for (int h = 0; h < KS / kSlab; ++h) cp_async16_or_zero((i % 2 ? odd : even) + to + h * slab_bytes + i / 2 * 1024u, at + (there ? h * kSlab : 0), there);
+                    }
+                    cp_async_commit();
+                    cp_async_wait_all();
+                    ptx::fence_proxy_async_smem();   // the copies are this thread's writes; tcgen05.mma reads shared memory through the asynchronous proxy
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(step_full(r.i));
+                    r.step(kLoadWarps, kSlots);
                 }
-                const uint32_t to = at + r.i * act_stride;
-                const uint16_t* from = p.x.a + l * KS + piece * 8u;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (16u * i >= act_rows) break;
-                    const bool there = src[i] < p.x.a_rows;
-                    const uint16_t* row = there ? from + (size_t)src[i] * p.x.lda : p.x.a;
-#pragma unroll
-                    for (int h = 0; h < KS / kSlab; ++h) cp_async16_or_zero(to + h * slab_bytes + i * 2048u, row + (there ? h * kSlab : 0), there);
-                }
-                cp_async_commit();
-                ++pending;
-                issued |= 1u << r.i; parity = (parity & ~(1u << r.i)) | (r.phase << r.i);
-                r.step(1, kSlots);
-                if (pending > 2) { cp_async_wait_but2(); report(); }
+                before += ns;
             }
+            // not while a commit of rank 0 may still arrive here: the last use of each slot, whoever's it was
+            for (uint32_t s = 0; who == 0 && ok && s < kSlots && s < before; ++s) (void)warp_wait(step_empty(s), (before - 1 - s) / kSlots & 1u, abort_flag);
+        } else {
+            // A lane copies 16 bytes of rows 16 * i + 4 * (which loader) + lane / 8 of this CTA's half, per 64 k.
+            const uint32_t r8 = (uint32_t)(warp - kFirstLoad) * 4 + ((uint32_t)lane >> 3), piece = (uint32_t)lane & 7u;
+            const uint32_t at = smem_base + off_act + r8 * 128u + ((piece ^ (r8 & 7u)) << 4);   // 16 rows on: the same place in the swizzle
+            Ring r{0, 0}, rp{0, 0};       // of the step that comes next, of the oldest one that has not been reported
+            uint32_t pending = 0, issued = 0, parity = 0;
+            bool ok = true;
+            // The copies are this thread's writes; tcgen05.mma reads shared memory through the asynchronous proxy.
+            auto report = [&] {
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(step_full(rp.i));
+                rp.step(1, kSlots);
+                --pending;
+            };
+            while (ok && next(x)) {
+                const uint32_t act_rows = x.height / 2, slab_bytes = act_rows * 128u;   // act_rows: a multiple of 16
+                uint32_t src[8];
+    #pragma unroll
+                for (int i = 0; i < 8; ++i) {   // rows behind the last one, and those that A does not have: zeros
+                    const uint32_t r0 = 16u * i + r8, c = rank * act_rows + r0;
+                    src[i] = r0 < act_rows && c < x.rows ? source_row(p.x, x.row0 + c) : 0xffffffffu;
+                }
+                for (uint32_t l = 0; l < ns; ++l) {
+                    // a free slot: go on; otherwise first report all that is under way
+                    if (!__all_sync(0xffffffffu, ptx::mbar_test_wait(step_empty(r.i), r.phase ^ 1u))) {
+                        if (pending) { cp_async_wait_all(); while (pending) report(); }
+                        if (!warp_wait(step_empty(r.i), r.phase ^ 1u, abort_flag)) { give_up(62, x.expert, l); ok = false; break; }
+                    }
+                    const uint32_t to = at + r.i * act_stride;
+                    const uint16_t* from = p.x.a + l * KS + piece * 8u;
+    #pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (16u * i >= act_rows) break;
+                        const bool there = src[i] < p.x.a_rows;
+                        const uint16_t* row = there ? from + (size_t)src[i] * p.x.lda : p.x.a;
+    #pragma unroll
+                        for (int h = 0; h < KS / kSlab; ++h) cp_async16_or_zero(to + h * slab_bytes + i * 2048u, row + (there ? h * kSlab : 0), there);
+                    }
+                    cp_async_commit();
+                    ++pending;
+                    issued |= 1u << r.i; parity = (parity & ~(1u << r.i)) | (r.phase << r.i);
+                    r.step(1, kSlots);
+                    if (pending > 2) { cp_async_wait_but2(); report(); }
+                }
+            }
+            cp_async_wait_all();
+            while (pending) report();
+            for (uint32_t s = 0; s < kSlots; ++s)   // not while a commit of rank 0 may still arrive here
+                if (issued & (1u << s)) (void)warp_wait(step_empty(s), (parity >> s) & 1u, abort_flag);
         }
-        cp_async_wait_all();
-        while (pending) report();
-        for (uint32_t s = 0; s < kSlots; ++s)   // not while a commit of rank 0 may still arrive here
-            if (issued & (1u << s)) (void)warp_wait(step_empty(s), (parity >> s) & 1u, abort_flag);
     } else {
         // ======================= epilogue =======================
         ptx::regs_up<regs_epi(CG)>();
         const uint32_t quarter = (uint32_t)warp & 3u, half = (uint32_t)(warp - kFirstEpi) >> 2, ch = quarter * 32 + lane;
-        constexpr int kPacks = 8;   // of 16 columns: this warp's half of a strip
+        constexpr int kPacks = LOW ? 2 : 8;   // of 16 columns: this warp's half of a strip
         const bool odd = lane & 1, gated = p.x.gated != 0, act = p.x.silu != 0;
         const uint32_t stage = smem_base + kOffOut + (uint32_t)(warp - kFirstEpi) * 2 * kOutBytes;
         Ring rc{0, 0};
         bool ok = true;
+        bool has[2] = {true, LOW};   // which issuers have had a step of the tile
+        uint32_t before = 0;         // steps of the tiles walked so far
         auto drained = [&] {   // everything of the accumulator is in registers
             ptx::tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) { if (rank == 0) ptx::mbar_arrive(acc_empty(rc.i)); else ptx::mbar_arrive_remote(acc_empty(rc.i), 0); }
+            if (lane == 0) {
+#pragma unroll
+                for (uint32_t h = 0; h < kIssuers; ++h) {
+                    const uint32_t b = acc_empty(kIssuers * rc.i + h);
+                    if (!has[h]) continue;
+                    if (rank == 0) ptx::mbar_arrive(b); else ptx::mbar_arrive_remote(b, 0);
+                }
+            }
         };
         auto pack2 = [](float lo, float hi) {
             const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -483,15 +537,29 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                 const uint32_t row = i * 32 + lane < valid ? p.x.row_pair ? source_row(p.x, x.row0 + first + i * 32 + lane) : x.row0 + first + i * 32 + lane : 0xffffffffu;
                 factor[i] = GROUPED && row < p.x.a_rows ? p.row_factor[row] * 512.f : 0.f;
             }
-            if (!warp_wait(acc_full(rc.i), rc.phase, abort_flag)) { give_up(68, x.expert, 0); break; }
+            if (LOW) { has[0] = ns > 1 || before % 2 == 0; has[1] = ns > 1 || before % 2 == 1; }
+            before += ns;
+            if (has[0] && !warp_wait(acc_full(kIssuers * rc.i), rc.phase, abort_flag)) { give_up(68, x.expert, 0); break; }
+            if (LOW && has[1] && !warp_wait(acc_full(2 * rc.i + 1), rc.phase, abort_flag)) { give_up(68, x.expert, 1); break; }
             ptx::tc_fence_after_sync();
 #pragma unroll
             for (int i = 0; i < kPacks; ++i) {
                 if (16u * i >= cols) break;
                 uint32_t a[16];
                 float v[16];
-                ptx::tmem_ld_32x16(column + rc.i * acc_cols + 16 * i, a);
-                ptx::tmem_ld_wait();
+                if (LOW) {   // the two issuers' sums
+                    uint32_t b[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) a[j] = b[j] = 0u;
+                    if (has[0]) ptx::tmem_ld_32x16(column + 2 * rc.i * acc_cols + 16 * i, a);
+                    if (has[1]) ptx::tmem_ld_32x16(column + (2 * rc.i + 1) * acc_cols + 16 * i, b);
+                    ptx::tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) + __uint_as_float(b[j]));
+                } else {
+                    ptx::tmem_ld_32x16(column + rc.i * acc_cols + 16 * i, a);
+                    ptx::tmem_ld_wait();
+                }
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
                     v[j] = GROUPED ? (__uint_as_float(a[j]) * scale) * __shfl_sync(0xffffffffu, factor[i / 2], i % 2 * 16 + j) : unscaled(__uint_as_float(a[j]), scale);
@@ -561,9 +629,9 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
     }
 }
 
-template <int BITS, bool GROUPED, int KS, int CG>
+template <int BITS, bool GROUPED, int KS, int CG, bool LOW>
 int launch_groups(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uint32_t smem, DeviceCtx* ctx, cudaStream_t s) {
-    auto kern = expert_many_kernel<BITS, GROUPED, KS, CG>;
+    auto kern = expert_many_kernel<BITS, GROUPED, KS, CG, LOW>;
     static DeviceOnce attr_set;  // per template instance
     if (!attr_set.done(ctx->device)) {
         cudaFuncAttributes attr;
@@ -587,7 +655,8 @@ int launch_groups(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uin
 
 template <int BITS, bool GROUPED, int KS>
 int launch_cfg(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uint32_t smem, DeviceCtx* ctx, cudaStream_t s) {
-    return p.x.tile_rows <= 128 ? launch_groups<BITS, GROUPED, KS, 4>(tw, p, grid, smem, ctx, s) : launch_groups<BITS, GROUPED, KS, 2>(tw, p, grid, smem, ctx, s);
+    if (p.x.tile_rows <= 64) return launch_groups<BITS, GROUPED, KS, 4, true>(tw, p, grid, smem, ctx, s);
+    return p.x.tile_rows <= 128 ? launch_groups<BITS, GROUPED, KS, 4, false>(tw, p, grid, smem, ctx, s) : launch_groups<BITS, GROUPED, KS, 2, false>(tw, p, grid, smem, ctx, s);
 }
 
 }  // namespace
@@ -597,18 +666,24 @@ int launch_expert_many(const ExpertParams& q, uint32_t bits, uint32_t group, Dev
     ManyParams p{};
     p.x = q;
     const uint32_t ks = q.k % 128 == 0 && group % 128 == 0 ? 128 : 64, spb = (bits == 8 ? 128 : 256) / ks, kSlots = slots(ks);
-    // up to 128 rows there are two accumulators, and twice the raw blocks under way
-    p.x.tile_rows = (uint64_t)q.m <= 160ull * q.experts ? 128 : 256;
     p.x.n_blocks = (q.n + 2 * kCh - 1) / (2 * kCh);
     p.steps = q.k / ks;
+    const uint32_t per_block = p.steps % spb == 0 ? spb : 1;
+    // up to 128 rows there are two accumulators, and twice the raw blocks under way; up to 64 two for each of two issuers (whole raw blocks only:
+    // see below)
+    p.x.tile_rows = (uint64_t)q.m <= 40ull * q.experts && per_block == spb ? 64 : (uint64_t)q.m <= 160ull * q.experts ? 128 : 256;
+    const bool low = p.x.tile_rows <= 64;
     p.accs = p.x.tile_rows <= 128 ? 2 : 1;
     p.off_raw = (kOffTable + ExpertTable::bytes(q.experts) + 1023u) / 1024u * 1024u;
     const uint32_t act_bytes = kSlots * p.x.tile_rows * ks;
     p.raw_stages = (232448 - 1024 - p.off_raw - act_bytes) / kRawBytes;
     if (p.raw_stages > (uint32_t)kMaxRaw) p.raw_stages = kMaxRaw;
-    // the parity waits of the converters: see stream.cu
-    const uint32_t per_block = p.steps % spb == 0 ? spb : 1, kConvGroups = p.x.tile_rows <= 128 ? 4 : 2;
-    p.slot_first = p.raw_stages * per_block >= kConvGroups + kSlots + per_block - 1 ? 0u : 1u;
+    // The parity waits of the converters: see stream.cu.  With two issuers a free slot tells about every second step only; so of the raw blocks either
+    // every one has a step of each issuer, or the ring is of an even number of blocks with a step each, and the block that had its place in the
+    // ring before had one of the same issuer's.
+    const uint32_t kConvGroups = p.x.tile_rows <= 128 ? 4 : 2;
+    if (low && spb == 1) p.raw_stages &= ~1u;
+    p.slot_first = !low && p.raw_stages * per_block >= kConvGroups + kSlots + per_block - 1 ? 0u : 1u;
     if (p.raw_stages * per_block < kSlots + per_block - 1) return AFB_ERR_UNSUPPORTED;   // not with any size that this function takes
     p.c_vec = q.ldc % 8 == 0 && (uintptr_t)q.c % 16 == 0 && q.n_out % 8 == 0;
     p.status = ctx->status;

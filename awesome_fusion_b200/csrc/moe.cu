@@ -13,8 +13,9 @@
 namespace afb {
 namespace {
 
-constexpr int kOneThreads = 512, kOneWarps = kOneThreads / 32, kRouteThreads = 1024, kRouteWarps = kRouteThreads / 32;
-constexpr uint32_t kOneBlockPairs = 512;   // up to here one CTA: its ranks are counted pair against pair
+constexpr int kRouteThreads = 1024, kRouteWarps = kRouteThreads / 32;
+// Up to here one CTA: two tokens a warp, ranks counted pair against pair (221 tokens of 108 experts, one pick: 22.5 us in one CTA).
+constexpr uint32_t kOneBlockTokens = 64, kOneBlockPairs = 512;
 constexpr uint32_t kMaxBlocks = 256;       // of the two-kernel form: every block reads all blocks' counts
 constexpr uint32_t kMinBlockTokens = 32;   // one per warp
 
@@ -101,13 +102,13 @@ __device__ __forceinline__ void scan_experts(const int32_t* count, int32_t* star
 }
 
 template <int NV>
-__global__ void __launch_bounds__(kOneThreads) route_one_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(kRouteThreads) route_one_kernel(const RouteParams p) {
     __shared__ int32_t s_id[kOneBlockPairs];
     __shared__ int32_t s_count[AFB_MOE_MAX_EXPERTS], s_start[AFB_MOE_MAX_EXPERTS + 1];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, pairs = p.tokens * p.top_k;
-    for (uint32_t e = tid; e < p.experts; e += kOneThreads) s_count[e] = 0;
+    for (uint32_t e = tid; e < p.experts; e += kRouteThreads) s_count[e] = 0;
     __syncthreads();
-    for (uint32_t t = warp; t < p.tokens; t += kOneWarps) {
+    for (uint32_t t = warp; t < p.tokens; t += kRouteWarps) {
         int32_t id; float w;
         pick_token<NV>(p, t, lane, id, w);
         if (lane < p.top_k) {
@@ -121,9 +122,9 @@ __global__ void __launch_bounds__(kOneThreads) route_one_kernel(const RouteParam
     __syncthreads();
     if (warp == 0) scan_experts(s_count, s_start, p.experts, lane);
     __syncthreads();
-    for (uint32_t e = tid; e <= p.experts; e += kOneThreads) p.offsets[e] = s_start[e];
+    for (uint32_t e = tid; e <= p.experts; e += kRouteThreads) p.offsets[e] = s_start[e];
     const uint32_t rows = (uint32_t)s_start[p.experts];
-    for (uint32_t i = tid; i < pairs; i += kOneThreads) {
+    for (uint32_t i = tid; i < pairs; i += kRouteThreads) {
         const int32_t id = s_id[i];
         int32_t row = -1;
         if (id >= 0) {
@@ -231,6 +232,8 @@ __global__ void clear_offsets_kernel(int32_t* offsets, uint32_t n) {
     for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) offsets[i] = 0;
 }
 
+bool one_block(uint32_t tokens, uint32_t top_k) { return tokens <= kOneBlockTokens && tokens * top_k <= kOneBlockPairs; }
+
 // Blocks of the two-kernel form: at most kMaxBlocks, of a multiple of kMinBlockTokens tokens.
 uint32_t route_block_tokens(uint32_t tokens) {
     const uint32_t least = (tokens + kMaxBlocks - 1) / kMaxBlocks;
@@ -239,8 +242,8 @@ uint32_t route_block_tokens(uint32_t tokens) {
 
 template <int NV>
 int launch_route(const RouteParams& p, DeviceCtx* ctx, cudaStream_t s) {
-    if ((uint64_t)p.tokens * p.top_k <= kOneBlockPairs) {
-        route_one_kernel<NV><<<1, kOneThreads, 0, s>>>(p);
+    if (one_block(p.tokens, p.top_k)) {
+        route_one_kernel<NV><<<1, kRouteThreads, 0, s>>>(p);
         count_launch();
         const cudaError_t e = cudaGetLastError();
         return e == cudaSuccess ? AFB_OK : cuda_fail(e);
@@ -352,7 +355,7 @@ extern "C" int afb_moe_route_workspace(uint32_t tokens, uint32_t experts, uint64
     if (!bytes || experts == 0 || experts > AFB_MOE_MAX_EXPERTS) return AFB_ERR_BAD_ARG;
     // also for sizes that one CTA takes: top_k decides, and it is not asked for here
     const uint64_t blocks = tokens ? (tokens + route_block_tokens(tokens) - 1) / route_block_tokens(tokens) : 0;
-    *bytes = (uint64_t)tokens * (experts < AFB_MOE_MAX_TOP_K ? experts : AFB_MOE_MAX_TOP_K) <= kOneBlockPairs ? 0 : blocks * experts * sizeof(int32_t);
+    *bytes = one_block(tokens, experts < AFB_MOE_MAX_TOP_K ? experts : AFB_MOE_MAX_TOP_K) ? 0 : blocks * experts * sizeof(int32_t);
     return AFB_OK;
 }
 
@@ -367,7 +370,7 @@ extern "C" int afb_moe_route_launch(const afb_moe_route_args* a, void* stream) {
             if (!ptr || (uintptr_t)ptr % 4) return AFB_ERR_BAD_ARG;
         if (!a->ptr_logits || (uintptr_t)a->ptr_logits % (a->logits_f32 ? 4 : 2)) return AFB_ERR_BAD_ARG;
         afb_moe_route_workspace(a->tokens, a->experts, &need);
-        if ((uint64_t)a->tokens * a->top_k > kOneBlockPairs && (!a->ptr_workspace || (uintptr_t)a->ptr_workspace % 4 || a->workspace_bytes < need)) return AFB_ERR_BAD_ARG;
+        if (!one_block(a->tokens, a->top_k) && (!a->ptr_workspace || (uintptr_t)a->ptr_workspace % 4 || a->workspace_bytes < need)) return AFB_ERR_BAD_ARG;
     }
     DeviceCtx* ctx = current_ctx();
     if (!ctx) return AFB_ERR_NOT_INIT;
