@@ -446,7 +446,7 @@ extern "C" int afb_expert_gemm_launch(const afb_expert_gemm_args* x, void* strea
     p.enc = a.b_encoding; p.scale_dtype = a.scale_dtype; p.packed = a.b_layout == AFB_LAYOUT_COL_PACKED ? 1u : 0u;
     for (uint32_t g = a.group_size; g > 1; g >>= 1) ++p.group_shift;
     p.gated = x->gated; p.silu = x->activation == AFB_ACT_SILU ? 1u : 0u;
-    const bool many = a.variant == AFB_VARIANT_PREFILL || (a.variant == AFB_VARIANT_AUTO && (uint64_t)a.m > (a.b_bits == 8 ? 10ull : 16ull) * x->experts);
+    const bool many = a.variant == AFB_VARIANT_PREFILL || (a.variant == AFB_VARIANT_AUTO && (uint64_t)a.m > (a.b_bits == 8 ? 4ull : 13ull) * x->experts);
     if (many && x->a_rows) {
         bool done = false;
         const int rc = launch_expert_many(p, a.b_bits, a.group_size, ctx, (cudaStream_t)stream, &done);

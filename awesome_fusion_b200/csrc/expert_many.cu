@@ -38,8 +38,8 @@ __host__ __device__ constexpr uint32_t regs_epi(int cg) { return cg == 4 ? 104 :
 __host__ __device__ constexpr uint32_t regs_conv(int cg) { return cg == 4 ? 56 : 64; }
 __host__ __device__ constexpr uint32_t regs_all(int cg) { return 128 * kRegsCtrl + 32 * kEpiWarps * regs_epi(cg) + 128 * cg * regs_conv(cg) + 32 * kLoadWarps * kRegsLoad; }
 static_assert(regs_all(2) <= 80u * many_threads(2) && regs_all(4) <= 64u * many_threads(4), "shares of the registers");
-constexpr int kMaxRaw = 12, kMaxSlots = 8, kMaxAcc = 4;
-__host__ __device__ constexpr uint32_t slots(int ks) { return ks == 128 ? 4 : 6; }   // steps under way, in 256 columns at most
+constexpr int kMaxRaw = 12, kMaxSlots = 8, kMaxAcc = 2;
+__host__ __device__ constexpr uint32_t slots(int ks, bool low) { return ks == 128 && !low ? 4 : 6; }   // steps under way, in 256 columns at most (low strips: 384)
 constexpr uint32_t kTmemCols = 512;
 constexpr int kBars = 2 * (kMaxRaw + kMaxSlots + kMaxAcc);
 constexpr int kOffMisc = kBars * 8, kOffOut = 1024;
@@ -100,6 +100,7 @@ struct PrepareParams {
 constexpr int kPrepareThreads = 256;
 __global__ void __launch_bounds__(kPrepareThreads) expert_prepare_kernel(const PrepareParams p) {
     const uint32_t lane = threadIdx.x & 31, id = blockIdx.x * (kPrepareThreads / 32) + (threadIdx.x >> 5);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the product's kernel sets up meanwhile; what this one writes it waits for
     if (id < p.x.a_rows) {
         const uint16_t* src = p.x.a + (size_t)id * p.x.lda;
         uint32_t most = 0;
@@ -156,7 +157,7 @@ __global__ void __launch_bounds__(many_threads(CG), 1)
 expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams p) {
     constexpr uint32_t SPB = (BITS == 8 ? 128 : 256) / KS;   // steps per raw block
     constexpr uint32_t kSlotCols = KS / 2;                   // TMEM columns of a step's weights
-    constexpr uint32_t kSlots = slots(KS);
+    constexpr uint32_t kSlots = slots(KS, LOW);
     constexpr int kConvGroups = CG, kFirstLoad = kFirstConv + 4 * CG;
     constexpr uint32_t kIssuers = LOW ? 2 : 1;
     static_assert(!LOW || (CG == 4 && kSlots % 2 == 0), "a slot's steps are one issuer's");
@@ -182,7 +183,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
     if (warp == 0 && lane == 0) {
         for (uint32_t s = 0; s < p.raw_stages; ++s) { ptx::mbar_init(raw_full(s), 1); ptx::mbar_init(raw_empty(s), 4 * SPB); }
         for (uint32_t s = 0; s < kSlots; ++s) { ptx::mbar_init(step_full(s), 4 + (LOW ? 1 : kLoadWarps) + (rank == 0 ? 1 : 0)); ptx::mbar_init(step_empty(s), 1); }
-        for (uint32_t s = 0; s < p.accs * kIssuers; ++s) { ptx::mbar_init(acc_full(s), 1); ptx::mbar_init(acc_empty(s), 2 * kEpiWarps); }
+        for (uint32_t s = 0; s < (LOW ? 2u : p.accs); ++s) { ptx::mbar_init(acc_full(s), 1); ptx::mbar_init(acc_empty(s), 2 * kEpiWarps); }
         *abort_flag = 0;
         ptx::fence_mbar_init();
         ptx::prefetch_tmap(&tmap_w);
@@ -198,6 +199,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
     ptx::cluster_arrive();
     ptx::cluster_wait();   // both CTAs' barriers are there
     ptx::tc_fence_after_sync();
+    if (GROUPED && warp >= kFirstEpi) asm volatile("griddepcontrol.wait;" ::: "memory");   // the warps before these touch weights only
     constexpr uint32_t tmem_base = 0;   // all 512 columns are this CTA's: the allocation starts at column 0
     const uint32_t slot_base = tmem_base + kTmemCols - kSlots * kSlotCols;   // accumulators from column 0, slots at the end
     const uint32_t acc_cols = p.x.tile_rows;
@@ -245,15 +247,13 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
             const uint32_t who = (uint32_t)warp - 2;
             const uint64_t desc0 = ptx::umma_desc_kmajor_sw128(smem_base + off_act);
             r.i = who;
-            Ring rc{0, 0};       // of the accumulator, or of this issuer's of a tile's two
+            Ring rc{0, 0};
             uint32_t before = 0, g = who;   // steps of the tiles walked so far; this warp's next step, counted over all tiles
             bool ready = false;
             while (ok && next(x)) {
                 const uint32_t idesc = GROUPED ? ptx::umma_idesc_f16_f32(2 * kCh, x.height) : ptx::umma_idesc_bf16_f32(2 * kCh, x.height), slab_d = x.height * 64u >> 4;
-                const uint32_t acc = LOW ? 2 * rc.i + who : rc.i, td = tmem_base + acc * acc_cols, acc_done = acc_full(acc), first = g;
-                if (g < before + ns) {   // of a tile of one step one of the two issuers has none
-                    if (!warp_wait(acc_empty(acc), rc.phase ^ 1u, abort_flag)) { give_up(63, x.expert, 0); break; }
-                }
+                const uint32_t acc = LOW ? who : rc.i, td = tmem_base + acc * acc_cols, acc_done = acc_full(acc), first = g;
+                if (!warp_wait(acc_empty(acc), rc.phase ^ 1u, abort_flag)) { give_up(63, x.expert, 0); break; }
                 for (; g < before + ns; g += kIssuers) {
                     if (!__all_sync(0xffffffffu, ready) && !warp_wait(step_full(r.i), r.phase, abort_flag)) { give_up(64, x.expert, g); ok = false; break; }
                     ptx::tc_fence_after_sync();
@@ -482,16 +482,13 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
         const uint32_t stage = smem_base + kOffOut + (uint32_t)(warp - kFirstEpi) * 2 * kOutBytes;
         Ring rc{0, 0};
         bool ok = true;
-        bool has[2] = {true, LOW};   // which issuers have had a step of the tile
-        uint32_t before = 0;         // steps of the tiles walked so far
         auto drained = [&] {   // everything of the accumulator is in registers
             ptx::tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) {
 #pragma unroll
                 for (uint32_t h = 0; h < kIssuers; ++h) {
-                    const uint32_t b = acc_empty(kIssuers * rc.i + h);
-                    if (!has[h]) continue;
+                    const uint32_t b = acc_empty(LOW ? h : rc.i);
                     if (rank == 0) ptx::mbar_arrive(b); else ptx::mbar_arrive_remote(b, 0);
                 }
             }
@@ -537,10 +534,8 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                 const uint32_t row = i * 32 + lane < valid ? p.x.row_pair ? source_row(p.x, x.row0 + first + i * 32 + lane) : x.row0 + first + i * 32 + lane : 0xffffffffu;
                 factor[i] = GROUPED && row < p.x.a_rows ? p.row_factor[row] * 512.f : 0.f;
             }
-            if (LOW) { has[0] = ns > 1 || before % 2 == 0; has[1] = ns > 1 || before % 2 == 1; }
-            before += ns;
-            if (has[0] && !warp_wait(acc_full(kIssuers * rc.i), rc.phase, abort_flag)) { give_up(68, x.expert, 0); break; }
-            if (LOW && has[1] && !warp_wait(acc_full(2 * rc.i + 1), rc.phase, abort_flag)) { give_up(68, x.expert, 1); break; }
+            if (!warp_wait(acc_full(rc.i), rc.phase, abort_flag)) { give_up(68, x.expert, 0); break; }
+            if (LOW && !warp_wait(acc_full(1), rc.phase, abort_flag)) { give_up(68, x.expert, 1); break; }
             ptx::tc_fence_after_sync();
 #pragma unroll
             for (int i = 0; i < kPacks; ++i) {
@@ -549,10 +544,8 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                 float v[16];
                 if (LOW) {   // the two issuers' sums
                     uint32_t b[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) a[j] = b[j] = 0u;
-                    if (has[0]) ptx::tmem_ld_32x16(column + 2 * rc.i * acc_cols + 16 * i, a);
-                    if (has[1]) ptx::tmem_ld_32x16(column + (2 * rc.i + 1) * acc_cols + 16 * i, b);
+                    ptx::tmem_ld_32x16(column + 16 * i, a);
+                    ptx::tmem_ld_32x16(column + acc_cols + 16 * i, b);
                     ptx::tmem_ld_wait();
 #pragma unroll
                     for (int j = 0; j < 16; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) + __uint_as_float(b[j]));
@@ -644,10 +637,12 @@ int launch_groups(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uin
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid); cfg.blockDim = dim3(many_threads(CG)); cfg.stream = s; cfg.dynamicSmemBytes = smem;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr; cfg.numAttrs = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // group scales: after expert_prepare_kernel
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = GROUPED ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, p);
     count_launch();
     return e == cudaSuccess ? AFB_OK : cuda_fail(e);
@@ -665,15 +660,17 @@ int launch_expert_many(const ExpertParams& q, uint32_t bits, uint32_t group, Dev
     *done = false;
     ManyParams p{};
     p.x = q;
-    const uint32_t ks = q.k % 128 == 0 && group % 128 == 0 ? 128 : 64, spb = (bits == 8 ? 128 : 256) / ks, kSlots = slots(ks);
+    const uint32_t ks = q.k % 128 == 0 && group % 128 == 0 ? 128 : 64, spb = (bits == 8 ? 128 : 256) / ks;
     p.x.n_blocks = (q.n + 2 * kCh - 1) / (2 * kCh);
     p.steps = q.k / ks;
     const uint32_t per_block = p.steps % spb == 0 ? spb : 1;
-    // up to 128 rows there are two accumulators, and twice the raw blocks under way; up to 64 two for each of two issuers (whole raw blocks only:
-    // see below)
-    p.x.tile_rows = (uint64_t)q.m <= 40ull * q.experts && per_block == spb ? 64 : (uint64_t)q.m <= 160ull * q.experts ? 128 : 256;
+    // Up to 128 rows there are two accumulators, and twice the raw blocks under way.  Up to 64 each of two issuers has one, in return for six slots (four, and two
+    // accumulators each: 843 cycles per step, of which the converters' turn, 2200 from a free slot to the next, is the most); whole raw blocks
+    // only (see below), and a step for each issuer.
+    p.x.tile_rows = (uint64_t)q.m <= 40ull * q.experts && per_block == spb && p.steps > 1 ? 64 : (uint64_t)q.m <= 160ull * q.experts ? 128 : 256;
     const bool low = p.x.tile_rows <= 64;
-    p.accs = p.x.tile_rows <= 128 ? 2 : 1;
+    const uint32_t kSlots = slots(ks, low);
+    p.accs = p.x.tile_rows <= 64 || p.x.tile_rows > 128 ? 1 : 2;
     p.off_raw = (kOffTable + ExpertTable::bytes(q.experts) + 1023u) / 1024u * 1024u;
     const uint32_t act_bytes = kSlots * p.x.tile_rows * ks;
     p.raw_stages = (232448 - 1024 - p.off_raw - act_bytes) / kRawBytes;
