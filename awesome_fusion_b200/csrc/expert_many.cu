@@ -89,65 +89,96 @@ __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((u
 // The factor that brings values of up to 2^(e + 1) below 2^15.
 __device__ __forceinline__ int headroom(int e) { return min(14 - e, 126); }
 
-// Group scales: the rows of A as fp16 with a power of two of their own, and the power of two of each channel's scales.  A warp takes a row, the
-// warps after them 32 channels each (of experts that have rows).
+// Group scales: the rows of A as fp16 with a power of two of their own, and the power of two of each channel's scales.  The first blocks take 256 channels each (of
+// experts that have rows), the others rows, with `row_threads` threads each, so that a row is held in registers between the search for its
+// largest value and the conversion: up to kHeld pieces of 16 bytes a thread, 16384 k with a block's 256 threads.
 struct PrepareParams {
     ExpertParams x;
     uint16_t* a;          // [a_rows, k]
     float* row_factor;    // what a row's products have to be multiplied by
     float* channel_mult;  // [experts * n] what a channel's scales are multiplied by
+    uint32_t channel_blocks, row_threads;
 };
-constexpr int kPrepareThreads = 256;
-__global__ void __launch_bounds__(kPrepareThreads) expert_prepare_kernel(const PrepareParams p) {
-    const uint32_t lane = threadIdx.x & 31, id = blockIdx.x * (kPrepareThreads / 32) + (threadIdx.x >> 5);
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the product's kernel sets up meanwhile; what this one writes it waits for
-    if (id < p.x.a_rows) {
-        const uint16_t* src = p.x.a + (size_t)id * p.x.lda;
-        uint32_t most = 0;
-#pragma unroll 4
-        for (uint32_t c = lane * 8; c < p.x.k; c += 256) {
-            const uint4 v = *reinterpret_cast<const uint4*>(src + c);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+constexpr int kPrepareThreads = 256, kHeld = 8;
+__device__ __forceinline__ uint32_t largest_finite(const uint4& v, uint32_t most) {   // as the bits of its absolute value
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t a = (w[i] >> (16 * h)) & 0x7fffu;
-                    if (a < 0x7f80u) most = max(most, a);   // infinities and NaN stay what they are
-                }
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t a = (w[i] >> (16 * h)) & 0x7fffu;
+            if (a < 0x7f80u) most = max(most, a);   // infinities and NaN stay what they are
         }
+    return most;
+}
+__device__ __forceinline__ uint4 to_f16(const uint4& v, float mult) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 h = __floats2half2_rn(__uint_as_float(w[i] << 16) * mult, __uint_as_float(w[i] & 0xffff0000u) * mult);
+        o[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
+}
+__global__ void __launch_bounds__(kPrepareThreads) expert_prepare_kernel(const PrepareParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the product's kernel sets up meanwhile; what this one writes it waits for
+    if (blockIdx.x >= p.channel_blocks) {
+        __shared__ uint32_t s_most[kPrepareThreads / 32];
+        const uint32_t per = p.row_threads, t = threadIdx.x % per, pieces = p.x.k / 8;
+        const uint64_t row = (uint64_t)(blockIdx.x - p.channel_blocks) * (kPrepareThreads / per) + threadIdx.x / per;
+        const bool there = row < p.x.a_rows;
+        const uint4* src = reinterpret_cast<const uint4*>(p.x.a + (there ? row : 0) * p.x.lda);
+        uint4* dst = reinterpret_cast<uint4*>(p.a + row * p.x.k);
+        uint4 held[kHeld];
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const uint32_t c = i * per + t;
+            held[i] = c < pieces ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) most = largest_finite(held[i], most);
+        for (uint32_t c = kHeld * per + t; c < pieces; c += per) most = largest_finite(src[c], most);
         most = __reduce_max_sync(0xffffffffu, most);
+        if (per > 32) {
+            if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = most;
+            __syncthreads();
+            for (uint32_t w = 0; w < per / 32; ++w) most = max(most, s_most[threadIdx.x / per * (per / 32) + w]);
+        }
+        if (!there) return;
         const int e = headroom(exponent_of(__uint_as_float(most << 16)));
         const float mult = power_of_two(e);
-        uint16_t* dst = p.a + (size_t)id * p.x.k;
-#pragma unroll 4
-        for (uint32_t c = lane * 8; c < p.x.k; c += 256) {
-            const uint4 v = *reinterpret_cast<const uint4*>(src + c);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-            uint32_t o[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const __half2 h = __floats2half2_rn(__uint_as_float(w[i] << 16) * mult, __uint_as_float(w[i] & 0xffff0000u) * mult);
-                o[i] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-            *reinterpret_cast<uint4*>(dst + c) = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int i = 0; i < kHeld; ++i) {
+            const uint32_t c = i * per + t;
+            if (c < pieces) dst[c] = to_f16(held[i], mult);
         }
-        if (lane == 0) p.row_factor[id] = power_of_two(-e);
+        for (uint32_t c = kHeld * per + t; c < pieces; c += per) dst[c] = to_f16(src[c], mult);
+        if (t == 0) p.row_factor[row] = power_of_two(-e);
         return;
     }
-    const uint64_t chan = (uint64_t)(id - p.x.a_rows) * 32 + lane, channels = (uint64_t)p.x.experts * p.x.n;
-    if (chan >= channels) return;
-    const uint32_t expert = (uint32_t)(chan / p.x.n);
+    const uint32_t chan = blockIdx.x * kPrepareThreads + threadIdx.x;
+    if (chan >= p.x.experts * p.x.n) return;
+    const uint32_t expert = chan / p.x.n, groups = p.x.k >> p.x.group_shift;
     if (clamp_offset(__ldg(p.x.offsets + expert + 1), p.x.m) <= clamp_offset(__ldg(p.x.offsets + expert), p.x.m)) return;
-    const uint32_t groups = p.x.k >> p.x.group_shift;
-    float most = 0.f;
+    float largest = 0.f;
+    if (p.x.scale_dtype == AFB_SCALE_BF16 && groups % 8 == 0 && (uintptr_t)p.x.scale % 16 == 0) {
+        const uint4* src = reinterpret_cast<const uint4*>(p.x.scale) + (size_t)chan * (groups / 8);
+        uint32_t most = 0;
+#pragma unroll 4
+        for (uint32_t g = 0; g < groups / 8; ++g) most = largest_finite(src[g], most);
+        largest = __uint_as_float(most << 16);
+    } else {
 #pragma unroll 8
-    for (uint32_t g = 0; g < groups; ++g) {
-        const float s = fabsf(p.x.scale_dtype == AFB_SCALE_BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.x.scale)[chan * groups + g] << 16)
-                                                                : reinterpret_cast<const float*>(p.x.scale)[chan * groups + g]);
-        if (s < INFINITY) most = fmaxf(most, s);
+        for (uint32_t g = 0; g < groups; ++g) {
+            const size_t at = (size_t)chan * groups + g;
+            const float s = fabsf(p.x.scale_dtype == AFB_SCALE_BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.x.scale)[at] << 16)
+                                                                    : reinterpret_cast<const float*>(p.x.scale)[at]);
+            if (s < INFINITY) largest = fmaxf(largest, s);
+        }
     }
-    p.channel_mult[chan] = power_of_two(headroom(exponent_of(most)));
+    p.channel_mult[chan] = power_of_two(headroom(exponent_of(largest)));
 }
 
 struct Strip : ExpertStrip { uint32_t n0; };   // n0: of this CTA's 128 channels
@@ -691,7 +722,7 @@ int launch_expert_many(const ExpertParams& q, uint32_t bits, uint32_t group, Dev
     if (group) {
         // rows of A, their factors, the channels' multipliers, each from a multiple of 256 bytes on
         const uint64_t a_bytes = ((uint64_t)q.a_rows * q.k * 2 + 255) / 256 * 256, row_bytes = ((uint64_t)q.a_rows * 4 + 255) / 256 * 256;
-        const uint64_t channels = (uint64_t)q.experts * q.n, warps = q.a_rows + (channels + 31) / 32;
+        const uint64_t channels = (uint64_t)q.experts * q.n;
         float* ws;
         uint32_t* counters;
         if (!stream_workspace(ctx, s, a_bytes + row_bytes + channels * 4, &ws, &counters)) return AFB_OK;
@@ -700,7 +731,10 @@ int launch_expert_many(const ExpertParams& q, uint32_t bits, uint32_t group, Dev
         prep.a = reinterpret_cast<uint16_t*>(ws);
         prep.row_factor = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + a_bytes);
         prep.channel_mult = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + a_bytes + row_bytes);
-        expert_prepare_kernel<<<(uint32_t)((warps + kPrepareThreads / 32 - 1) / (kPrepareThreads / 32)), kPrepareThreads, 0, s>>>(prep);
+        prep.channel_blocks = (uint32_t)((channels + kPrepareThreads - 1) / kPrepareThreads);
+        for (prep.row_threads = 32; prep.row_threads < (uint32_t)kPrepareThreads && prep.row_threads * kHeld * 8 < q.k;) prep.row_threads *= 2;
+        const uint32_t rows = kPrepareThreads / prep.row_threads;
+        expert_prepare_kernel<<<prep.channel_blocks + (q.a_rows + rows - 1) / rows, kPrepareThreads, 0, s>>>(prep);
         count_launch();
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) { *done = true; return cuda_fail(e); }
