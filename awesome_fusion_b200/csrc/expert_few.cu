@@ -446,7 +446,11 @@ extern "C" int afb_expert_gemm_launch(const afb_expert_gemm_args* x, void* strea
     p.enc = a.b_encoding; p.scale_dtype = a.scale_dtype; p.packed = a.b_layout == AFB_LAYOUT_COL_PACKED ? 1u : 0u;
     for (uint32_t g = a.group_size; g > 1; g >>= 1) ++p.group_shift;
     p.gated = x->gated; p.silu = x->activation == AFB_ACT_SILU ? 1u : 0u;
-    const bool many = a.variant == AFB_VARIANT_PREFILL || (a.variant == AFB_VARIANT_AUTO && (uint64_t)a.m > (a.b_bits == 8 ? 4ull : 13ull) * x->experts);
+    // Which form is the faster one, by the mean of the rows per expert (us, few / many; their own numbers of rows spread around it):
+    //   64 experts of 2048 x 4096 gated, int4 group-128: 8 rows 90 / 105, 12: 116 / 122, 16: 137 / 121, 24: 170 / 136;  int8: 4: 84 / 82, 8: 105 / 92
+    //   8 of 11008 x 4096, int4 group-128: 12: 78 / 89, 16: 92 / 91, 24: 125 / 91;  int8: 4: 84 / 80, 12: 90 / 81
+    //   16 of 4096 x 2816, int4 group-64: 8: 51 / 58, 12: 61 / 58, 24: 84 / 60;  128 of 1536 x 2048, int8 group-128: 4: 76 / 81, 8: 96 / 89
+    const bool many = a.variant == AFB_VARIANT_PREFILL || (a.variant == AFB_VARIANT_AUTO && (uint64_t)a.m > (a.b_bits == 8 ? 4ull : 12ull) * x->experts);
     if (many && x->a_rows) {
         bool done = false;
         const int rc = launch_expert_many(p, a.b_bits, a.group_size, ctx, (cudaStream_t)stream, &done);

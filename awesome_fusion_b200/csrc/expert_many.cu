@@ -333,22 +333,32 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
         const uint32_t mul0 = BITS == 8 ? (GROUPED ? kByteF16 : kMulByte) : !GROUPED ? nib.mul[0] : p.x.packed ? kByteF16 : kPairF16;
         const uint32_t mul1 = BITS == 8 ? mul0 : !GROUPED ? nib.mul[1] : p.x.packed ? kHighF16 : kPairF16;
         auto unpack2 = [&](uint32_t v, uint32_t mul, uint32_t add, uint32_t sc) { return GROUPED ? f16x2_mul(f16x2_fma(v, mul, add), sc) : bf16x2_fma(v, mul, add); };
-        uint32_t add = add_of(0);
+        uint32_t add[KS / 64];
+#pragma unroll
+        for (int h = 0; h < KS / 64; ++h) add[h] = add_of(0);
         const uint32_t row = p.off_raw + ch * 128, swz = (ch & 7u) << 4, lanes = (quarter * 32u) << 16;
         uint32_t steps_before = 0, blocks_before = 0;   // of the tiles walked so far
         bool ok = true;
         while (ok && next(x)) {
             const uint32_t nn = x.n0 + ch;
             const size_t chan = (size_t)x.expert * p.x.n + (nn < p.x.n ? nn : 0);
-            if (!GROUPED && has_zero) add = add_of(zero_of(chan));
+            if (!GROUPED && has_zero) {
+#pragma unroll
+                for (int h = 0; h < KS / 64; ++h) add[h] = add_of(zero_of(chan));
+            }
             const float mult = GROUPED ? p.channel_mult[chan] : 1.f;
-            // scale and zero-point of this group's next step, as they are stored
-            uint32_t sc_nxt = 0, z_nxt = 0;
+            // scales and zero-points of this group's next step, of each 64 k, as they are stored
+            uint32_t sc_nxt[KS / 64] = {}, z_nxt[KS / 64] = {};
             auto load_group = [&](uint32_t l) {
-                if (!GROUPED || l >= ns) return;
-                const size_t i = chan * groups_per_row + ((l * KS) >> p.x.group_shift);
-                sc_nxt = p.x.scale_dtype == AFB_SCALE_BF16 ? reinterpret_cast<const uint16_t*>(p.x.scale)[i] : reinterpret_cast<const uint32_t*>(p.x.scale)[i];
-                if (has_zero) z_nxt = p.x.zero[i];
+                if constexpr (GROUPED) {
+                    if (l >= ns) return;
+#pragma unroll
+                    for (int h = 0; h < KS / 64; ++h) {
+                        const size_t i = chan * groups_per_row + ((l * KS + h * 64) >> p.x.group_shift);
+                        sc_nxt[h] = p.x.scale_dtype == AFB_SCALE_BF16 ? reinterpret_cast<const uint16_t*>(p.x.scale)[i] : reinterpret_cast<const uint32_t*>(p.x.scale)[i];
+                        if (has_zero) z_nxt[h] = p.x.zero[i];
+                    }
+                }
             };
             uint32_t l = (g - steps_before) & (kConvGroups - 1);
             Ring rr, rs;
@@ -357,10 +367,13 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
             load_group(l);
             for (; l < ns; l += kConvGroups) {
                 const uint32_t sub = l % SPB;
-                uint32_t sc = 0;
+                uint32_t sc[KS / 64] = {};
                 if (GROUPED) {
-                    sc = f16_dup(__uint_as_float(p.x.scale_dtype == AFB_SCALE_BF16 ? sc_nxt << 16 : sc_nxt) * mult);
-                    if (has_zero) add = add_of(BITS == 8 ? decode_zero8(z_nxt, p.x.enc) : decode_zero4(z_nxt, p.x.enc));
+#pragma unroll
+                    for (int h = 0; h < KS / 64; ++h) {
+                        sc[h] = f16_dup(__uint_as_float(p.x.scale_dtype == AFB_SCALE_BF16 ? sc_nxt[h] << 16 : sc_nxt[h]) * mult);
+                        if (has_zero) add[h] = add_of(BITS == 8 ? decode_zero8(z_nxt[h], p.x.enc) : decode_zero4(z_nxt[h], p.x.enc));
+                    }
                     load_group(l + kConvGroups);
                 }
                 if (p.slot_first && !warp_wait(step_empty(rs.i), rs.phase ^ 1u, abort_flag)) { give_up(66, x.expert, l); ok = false; break; }
@@ -379,17 +392,18 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
 #pragma unroll
                     for (int q = 0; q < kWords / kPerStore; ++q) {
                         uint32_t o[16];
+                        const int k64 = BITS == 8 ? h : q / 2;   // which 64 k of the step
 #pragma unroll
                         for (int j = 0; j < kPerStore; ++j) {
                             const uint32_t v = w[q * kPerStore + j];
                             if (BITS == 8) {
                                 const uint32_t t8 = v ^ flip;
-                                o[2 * j] = unpack2(prmt(t8, 0u, sel0), mul0, add, sc);
-                                o[2 * j + 1] = unpack2(prmt(t8, 0u, sel1), mul0, add, sc);
+                                o[2 * j] = unpack2(prmt(t8, 0u, sel0), mul0, add[k64], sc[k64]);
+                                o[2 * j + 1] = unpack2(prmt(t8, 0u, sel1), mul0, add[k64], sc[k64]);
                             } else {   // s4x8_to_bf16's steps
                                 const uint32_t e = lop3_and_xor(v, 0x0f0f0f0fu, flip & 0x0f0f0f0fu), d = lop3_and_xor(v, 0xf0f0f0f0u, flip & 0xf0f0f0f0u);
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) o[4 * j + i] = unpack2(prmt(e, d, nib.sel[i]), i % 2 ? mul1 : mul0, add, sc);
+                                for (int i = 0; i < 4; ++i) o[4 * j + i] = unpack2(prmt(e, d, nib.sel[i]), i % 2 ? mul1 : mul0, add[k64], sc[k64]);
                             }
                         }
                         if (h == 0 && q == 0) {
@@ -691,7 +705,7 @@ int launch_expert_many(const ExpertParams& q, uint32_t bits, uint32_t group, Dev
     *done = false;
     ManyParams p{};
     p.x = q;
-    const uint32_t ks = q.k % 128 == 0 && group % 128 == 0 ? 128 : 64, spb = (bits == 8 ? 128 : 256) / ks;
+    const uint32_t ks = q.k % 128 == 0 ? 128 : 64, spb = (bits == 8 ? 128 : 256) / ks;
     p.x.n_blocks = (q.n + 2 * kCh - 1) / (2 * kCh);
     p.steps = q.k / ks;
     const uint32_t per_block = p.steps % spb == 0 ? spb : 1;
@@ -745,8 +759,7 @@ int launch_expert_many(const ExpertParams& q, uint32_t bits, uint32_t group, Dev
     CUtensorMap tw;
     const int rc = tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.b, (uint64_t)q.k * bits / 8, (uint64_t)q.experts * q.n, q.ldb_bytes, 128, kCh, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
-    if (bits == 4 && !group) return launch_cfg<4, false, 128>(tw, p, grid, smem, ctx, s);   // k is a multiple of 128
-    if (bits == 4) return ks == 128 ? launch_cfg<4, true, 128>(tw, p, grid, smem, ctx, s) : launch_cfg<4, true, 64>(tw, p, grid, smem, ctx, s);
+    if (bits == 4) return group ? launch_cfg<4, true, 128>(tw, p, grid, smem, ctx, s) : launch_cfg<4, false, 128>(tw, p, grid, smem, ctx, s);   // k is a multiple of 128
     if (group) return ks == 128 ? launch_cfg<8, true, 128>(tw, p, grid, smem, ctx, s) : launch_cfg<8, true, 64>(tw, p, grid, smem, ctx, s);
     return ks == 128 ? launch_cfg<8, false, 128>(tw, p, grid, smem, ctx, s) : launch_cfg<8, false, 64>(tw, p, grid, smem, ctx, s);
 }

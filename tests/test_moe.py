@@ -317,7 +317,8 @@ def test_expert_gemm_ragged(afb, variant, counts):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("variant", FORMS)
-@pytest.mark.parametrize("n, k, bits, group", [(1, 64, 8, 0), (7, 128, 4, 128), (128, 128, 4, 64), (129, 4160, 8, 64), (256, 14336, 4, 128), (3000, 192, 8, 0), (130, 8192, 8, 0)])
+@pytest.mark.parametrize("n, k, bits, group", [(1, 64, 8, 0), (7, 128, 4, 128), (128, 128, 4, 64), (129, 4160, 8, 64), (256, 14336, 4, 128), (3000, 192, 8, 0), (130, 8192, 8, 0), (40, 16512, 8, 64),
+                                              (200, 320, 8, 64), (200, 128, 8, 0), (64, 16640, 4, 64)])
 def test_expert_gemm_sizes_on_gpu(afb, variant, n, k, bits, group):
     x = Experts(3, n, k, bits, group, seed=7)
     counts = [20, 5, 61]
