@@ -91,8 +91,8 @@ __device__ __forceinline__ uint32_t source_row(const ExpertParams& p, uint32_t r
 
 __device__ __forceinline__ float silu(float v) { return v * sigmoid(v); }
 
-// `bits`, `group`: of the weights.  The form for many rows needs rows of A (a_rows > 0) and, for group scales, a workspace; *done = false: there is none
-// to be had, and nothing has happened.
+// `bits`, `group`: of the weights.  For group scales the form for many rows needs a workspace; *done = false: there is none to be had, and nothing has
+// happened.
 int launch_expert_many(const ExpertParams& p, uint32_t bits, uint32_t group, DeviceCtx* ctx, cudaStream_t s, bool* done);
 int launch_expert_few(const ExpertParams& p, uint32_t bits, uint32_t group, DeviceCtx* ctx, cudaStream_t s);
 

@@ -423,7 +423,7 @@ extern "C" int afb_expert_gemm_launch(const afb_expert_gemm_args* x, void* strea
     if (a.reserved != 0 || a.reserved2 != 0 || (a.b_bits != 8 && a.b_bits != 4) || a.b_encoding > 1 || a.b_layout > 2 || a.scale_dtype > 1 || a.variant > 3) return AFB_ERR_BAD_ARG;
     if (a.lda < a.k || a.ldb < a.k || a.ldc < n_out || (a.group_size && a.k % a.group_size)) return AFB_ERR_BAD_ARG;
     if (!a.ptr_b || !a.ptr_scale || (uintptr_t)a.ptr_scale % (a.scale_dtype == AFB_SCALE_BF16 ? 2 : 4) || (uintptr_t)a.ptr_c % 2 || (uintptr_t)a.ptr_a % 2) return AFB_ERR_BAD_ARG;
-    if (a.m && (!a.ptr_c || (x->a_rows && !a.ptr_a))) return AFB_ERR_BAD_ARG;
+    if (a.m && (!a.ptr_c || !a.ptr_a || !x->a_rows)) return AFB_ERR_BAD_ARG;
     if (a.m && !x->ptr_row_pair && x->a_rows < a.m) return AFB_ERR_BAD_ARG;
     if (a.flags || a.variant == AFB_VARIANT_NAIVE || a.b_layout == AFB_LAYOUT_ROW) return AFB_ERR_UNSUPPORTED;
     if (a.k % (a.b_bits == 8 ? 64u : 128u) || a.lda % 8 || ((uint64_t)a.ldb * a.b_bits / 8) % 16) return AFB_ERR_UNSUPPORTED;
@@ -451,7 +451,7 @@ extern "C" int afb_expert_gemm_launch(const afb_expert_gemm_args* x, void* strea
     //   8 of 11008 x 4096, int4 group-128: 12: 78 / 89, 16: 92 / 91, 24: 125 / 91;  int8: 4: 84 / 80, 12: 90 / 81
     //   16 of 4096 x 2816, int4 group-64: 8: 51 / 58, 12: 61 / 58, 24: 84 / 60;  128 of 1536 x 2048, int8 group-128: 4: 76 / 81, 8: 96 / 89
     const bool many = a.variant == AFB_VARIANT_PREFILL || (a.variant == AFB_VARIANT_AUTO && (uint64_t)a.m > (a.b_bits == 8 ? 4ull : 12ull) * x->experts);
-    if (many && x->a_rows) {
+    if (many) {
         bool done = false;
         const int rc = launch_expert_many(p, a.b_bits, a.group_size, ctx, (cudaStream_t)stream, &done);
         if (done) return rc;

@@ -265,7 +265,7 @@ typedef struct afb_expert_gemm_args {
     const int32_t* ptr_row_pair;   /* [m], or NULL  */
     uint32_t experts;              /* 1 .. AFB_MOE_MAX_EXPERTS */
     uint32_t top_k;                /* divisor of ptr_row_pair; 1 where it is NULL */
-    uint32_t a_rows;               /* rows of A */
+    uint32_t a_rows;               /* rows of A, 1 or more (where m is) */
     uint32_t gated;                /* 0 / 1 */
     uint32_t activation;           /* AFB_ACT_* */
     uint32_t reserved;             /* must be 0 */

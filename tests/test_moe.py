@@ -76,7 +76,7 @@ def _expert(lib, gemm=None, **changes):
     (dict(variant=4), {}), (dict(reserved=1), {}), (dict(reserved2=1), {}), (dict(group_size=96), {}), (dict(ptr_scale=PTR + 2), {}),
     (dict(ptr_c=PTR + 1), {}), (dict(ptr_a=PTR + 1), {}), ({}, dict(ptr_offsets=0)), ({}, dict(ptr_offsets=PTR + 2)), ({}, dict(ptr_row_pair=PTR + 1)),
     ({}, dict(experts=0)), ({}, dict(experts=1025)), ({}, dict(top_k=0)), ({}, dict(ptr_row_pair=0)), ({}, dict(gated=2)), ({}, dict(activation=2)),
-    ({}, dict(reserved=1)), (dict(n=255, ldc=255), dict(gated=1)), ({}, dict(ptr_row_pair=0, top_k=1, a_rows=15))])
+    ({}, dict(reserved=1)), (dict(n=255, ldc=255), dict(gated=1)), ({}, dict(ptr_row_pair=0, top_k=1, a_rows=15)), ({}, dict(a_rows=0))])
 def test_expert_gemm_refuses(lib, gemm, changes):
     assert _expert(lib, gemm, **changes) == E_BAD
 
@@ -349,6 +349,29 @@ def test_expert_gemm_strides_and_values(afb, variant):
     got = x.run(afb, a, offsets, variant=variant)
     keep = [r for r in range(rows) if r not in (5, 50)]
     assert torch.equal(got[keep], plain[keep]) and got[5].isnan().all() and not got[50].isfinite().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", FORMS)
+@pytest.mark.parametrize("fmt", [dict(bits=8), dict(bits=4, group=64, packed=True)], ids=lambda f: f"int{f['bits']}")
+def test_expert_gemm_pitch_of_weights_and_odd_gates(afb, variant, fmt):
+    """Rows of B with a pitch, an odd number of gated channels (no 4- or 8-byte store fits), a first row that is not row 0."""
+    x = Experts(3, 130, 384, seed=23, **fmt)
+    offsets = torch.tensor([4, 24, 24, 90], dtype=torch.int32, device="cuda")
+    a = activations(90, 384)
+    for gated in (False, True):
+        want = x.run(afb, a, offsets, gated=gated, variant=variant)
+        plain, off = x.plain(a, offsets, gated=gated, variant=variant)
+        check(want[4:], plain[4:], off[4:])
+        assert (want[:4] == 777).all()
+        wide = torch.randint(0, 255, (3, 130, x.b.shape[2] + 64), device="cuda").to(torch.uint8)
+        wide[:, :, : x.b.shape[2]] = x.b
+        out = torch.full_like(want, 777.0)
+        gemm = afb.make_args(out, a, wide, x.scale, 90, 130, 384, ldb=wide.shape[2] * 8 // x.bits, ldc=out.shape[1], bits=x.bits, group=x.group,
+                             layout=pkg.LAYOUT_COL_PACKED if x.packed else pkg.LAYOUT_COL, variant=variant,
+                             scale_dtype=pkg.SCALE_BF16 if x.group else pkg.SCALE_F32)
+        afb.expert_gemm_launch(afb.make_expert_gemm_args(gemm, offsets, experts=3, gated=gated, activation=pkg.ACT_SILU if gated else pkg.ACT_NONE))
+        assert torch.equal(out, want)
 
 
 @pytest.mark.gpu
