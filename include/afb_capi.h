@@ -136,7 +136,7 @@ int afb_device_sync(void);
  * so it must not run next to launches on that stream or to other graphs captured on it.
  * The streaming form of both variants (stream.cu: mostly 4 to 128 rows of large matrices) and the pair form (pair.cu: mostly from 65 rows,
  * and the fused launches) have workspaces of their own: one per stream for both (39 MB; afb_init allocates the first) and one per captured
- * graph (4 to 39 MB, by need): such graphs may run next to each other and to their capture stream.  The first 32 captured graphs
+ * graph (4 to 39 MB, by need; products grouped by expert up to 1 GB): such graphs may run next to each other and to their capture stream.  The first 32 captured graphs
  * keep theirs until afb_finalize; a further graph's goes back to the library when the graph and its executables are destroyed,
  * which costs its replays 2.5 us each.  (Two executables of ONE graph share its workspace; an executable
  * updated from another graph uses that graph's, which must then outlive it.)  They are allocated when first needed, also
