@@ -1,4 +1,4 @@
-// The activation of the fused epilogues (pair.cu, expert_few.cu, expert_many.cu).
+// The activation of the pair form's fused epilogue (pair.cu).
 #pragma once
 
 namespace afb {

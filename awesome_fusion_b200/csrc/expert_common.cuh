@@ -1,7 +1,6 @@
 // Shared by the two forms of the products grouped by expert (expert_few.cu, expert_many.cu): the parameter block and the table by which a CTA
 // finds its tiles.  How many rows an expert has is known on the GPU only.
 #pragma once
-#include "activation.cuh"
 #include "afb_internal.h"
 
 namespace afb {
@@ -89,7 +88,15 @@ __device__ __forceinline__ uint32_t source_row(const ExpertParams& p, uint32_t r
     return pair < 0 ? 0xffffffffu : (uint32_t)pair / p.top_k;
 }
 
-__device__ __forceinline__ float silu(float v) { return v * sigmoid(v); }
+// v / (1 + exp(-v)) for a result that is rounded to bf16: the product -v log2(e) is rounded once, so the exponential is off by |v| 2^-24 and a little (2^-17 at
+// |v| = 87, where it leaves fp32), a 500th of the rounding to come.  (sigmoid() of activation.cuh has three times the instructions: the drain of an accumulator of 256
+// gated columns waits for them.)  Below -128 infinity gives -0, at -infinity NaN, as the quotient would.
+__device__ __forceinline__ float silu(float v) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.44269504f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return v * r;
+}
 
 // `bits`, `group`: of the weights.  For group scales the form for many rows needs a workspace; *done = false: there is none to be had, and nothing has
 // happened.

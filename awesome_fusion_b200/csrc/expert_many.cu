@@ -549,7 +549,9 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
             // 16 finished sums of this lane's channel -> packed results.  Gated: the lanes of a pair hold gate (even) and up (odd) of one output
             // channel and exchange half of the 16 rows: the even lane finishes rows 0 to 7, the odd one 8 to 15.
             uint32_t o[kPacks][8];
-            auto finish = [&](uint32_t (&to)[8], const float (&v)[16]) {
+            float factor[4] = {};   // group scales: what rows lane, lane + 32, ... have to be multiplied by
+            auto row_scaled = [&](float v, uint32_t row) { return GROUPED ? v * __shfl_sync(0xffffffffu, factor[row / 32], row) : v; };
+            auto finish = [&](uint32_t (&to)[8], const float (&v)[16], int at) {   // at: the first of the 16 rows
                 if (gated) {
 #pragma unroll
                     for (int j = 0; j < 8; j += 2) {
@@ -557,14 +559,19 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const float lo = v[j + i], hi = v[j + i + 8], other = __shfl_xor_sync(0xffffffffu, odd ? lo : hi, 1);
-                            const float gate = odd ? other : lo, up = odd ? hi : other;
+                            // the two lanes of a pair have different rows: the factor is fetched from the lane that knows it
+                            const float fr = GROUPED ? __shfl_sync(0xffffffffu, factor[at / 32], at % 32 + j + i + (odd ? 8 : 0)) : 1.f;
+                            const float gate = (odd ? other : lo) * fr, up = (odd ? hi : other) * fr;
                             f[i] = (act ? silu(gate) : gate) * up;
                         }
                         to[j / 2] = pack2(f[0], f[1]);
                     }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) to[j] = pack2(act ? silu(v[2 * j]) : v[2 * j], act ? silu(v[2 * j + 1]) : v[2 * j + 1]);
+                    for (int j = 0; j < 8; ++j) {
+                        const float lo = row_scaled(v[2 * j], at + 2 * j), hi = row_scaled(v[2 * j + 1], at + 2 * j + 1);
+                        to[j] = pack2(act ? silu(lo) : lo, act ? silu(hi) : hi);
+                    }
                 }
             };
             const uint32_t column = tmem_base + ((quarter * 32u) << 16) + half * cols;
@@ -573,7 +580,6 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
             const float scale = GROUPED ? 1.f / p.channel_mult[chan]
                                         : p.x.scale_dtype == AFB_SCALE_BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.x.scale)[chan] << 16)
                                                                             : reinterpret_cast<const float*>(p.x.scale)[chan];
-            float factor[4];   // of rows lane, lane + 32, ...
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
                 const uint32_t row = i * 32 + lane < valid ? p.x.row_pair ? source_row(p.x, x.row0 + first + i * 32 + lane) : x.row0 + first + i * 32 + lane : 0xffffffffu;
@@ -600,8 +606,8 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                 }
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
-                    v[j] = GROUPED ? (__uint_as_float(a[j]) * scale) * __shfl_sync(0xffffffffu, factor[i / 2], i % 2 * 16 + j) : unscaled(__uint_as_float(a[j]), scale);
-                finish(o[i], v);
+                    v[j] = GROUPED ? __uint_as_float(a[j]) * scale : unscaled(__uint_as_float(a[j]), scale);
+                finish(o[i], v, 16 * i);
             }
             drained();
             rc.step(1, p.accs);
