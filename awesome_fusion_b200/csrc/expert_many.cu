@@ -64,8 +64,7 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
-__device__ __forceinline__ void cp_async_wait_but2() { asm volatile("cp.async.wait_group 2;" ::: "memory"); }
+template <uint32_t N> __device__ __forceinline__ void cp_async_wait_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }   // all but the newest N
 
 // Two fp16 values at a time.
 __device__ __forceinline__ uint32_t f16x2_mul(uint32_t a, uint32_t b) {
@@ -213,7 +212,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
 
     if (warp == 0 && lane == 0) {
         for (uint32_t s = 0; s < p.raw_stages; ++s) { ptx::mbar_init(raw_full(s), 1); ptx::mbar_init(raw_empty(s), 4 * SPB); }
-        for (uint32_t s = 0; s < kSlots; ++s) { ptx::mbar_init(step_full(s), 4 + (LOW ? 1 : kLoadWarps) + (rank == 0 ? 1 : 0)); ptx::mbar_init(step_empty(s), 1); }
+        for (uint32_t s = 0; s < kSlots; ++s) { ptx::mbar_init(step_full(s), 4 + kLoadWarps + (rank == 0 ? 1 : 0)); ptx::mbar_init(step_empty(s), 1); }
         for (uint32_t s = 0; s < (LOW ? 2u : p.accs); ++s) { ptx::mbar_init(acc_full(s), 1); ptx::mbar_init(acc_empty(s), 2 * kEpiWarps); }
         *abort_flag = 0;
         ptx::fence_mbar_init();
@@ -431,93 +430,55 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
         }
     } else if (warp >= kFirstLoad) {
         // ======================= rows of A =======================
+        // All four warps copy a step together and report it when they have issued kLag more, so that neither a copy's latency nor a slot's is waited for
+        // twice: with kSlots - kLag steps the tensor cores have enough.  (Each step waited for as soon as the next slot was not free yet: 1000 cycles a step,
+        // whatever its height.)  A lane copies 16 bytes of rows 16 * i + 4 * (which loader) + lane / 8 of this CTA's half, per 64 k.
         ptx::regs_down<kRegsLoad>();
-        if constexpr (LOW) {
-            // Low strips: each of the four warps takes every fourth step and waits for its copies, so that their latency is spread over four steps.  A lane
-            // copies 16 bytes of rows 4 * i + lane / 8 of this CTA's half, per 64 k; lane l knows where row l comes from.
-            const uint32_t who = (uint32_t)(warp - kFirstLoad), r4 = (uint32_t)lane >> 3, piece = (uint32_t)lane & 7u;
-            const uint32_t even = smem_base + off_act + r4 * 128u + ((piece ^ r4) << 4), odd = smem_base + off_act + (4 + r4) * 128u + ((piece ^ (4 + r4)) << 4);
-            Ring r{who, 0};
-            uint32_t before = 0, g = who;   // g: this warp's next step, counted over all tiles
-            bool ok = true;
-            while (ok && next(x)) {
-                const uint32_t act_rows = x.height / 2, slab_bytes = act_rows * 128u, c = rank * act_rows + lane;   // act_rows: 16 or 32
-                const uint32_t src = (uint32_t)lane < act_rows && c < x.rows ? source_row(p.x, x.row0 + c) : 0xffffffffu;   // none: zeros
-                for (; g < before + ns; g += kLoadWarps) {
-                    if (!warp_wait(step_empty(r.i), r.phase ^ 1u, abort_flag)) { give_up(62, x.expert, g); ok = false; break; }
-                    const uint32_t to = r.i * act_stride;
-                    const uint16_t* from = p.x.a + (g - before) * KS + piece * 8u;
+        constexpr uint32_t kLag = kSlots / 2 - 1;
+        const uint32_t r8 = (uint32_t)(warp - kFirstLoad) * 4 + ((uint32_t)lane >> 3), piece = (uint32_t)lane & 7u;
+        const uint32_t at = smem_base + off_act + r8 * 128u + ((piece ^ (r8 & 7u)) << 4);   // 16 rows on: the same place in the swizzle
+        Ring r{0, 0}, rp{0, 0};       // of the step that comes next, of the oldest one that has not been reported
+        uint32_t pending = 0, issued = 0, parity = 0;
+        bool ok = true;
+        // The copies are this thread's writes; tcgen05.mma reads shared memory through the asynchronous proxy.
+        auto report = [&] {
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(step_full(rp.i));
+            rp.step(1, kSlots);
+            --pending;
+        };
+        while (ok && next(x)) {
+            const uint32_t act_rows = x.height / 2, slab_bytes = act_rows * 128u;   // act_rows: a multiple of 16
+            constexpr int kTurns = LOW ? 2 : 8;
+            uint32_t src[kTurns];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if (4u * i >= act_rows) break;
-                        const uint32_t row = __shfl_sync(0xffffffffu, src, i * 4 + r4);
-                        const bool there = row < p.x.a_rows;
-                        const uint16_t* at = there ? from + (size_t)row * p.x.lda : p.x.a;
+            for (int i = 0; i < kTurns; ++i) {   // rows behind the last one, and those that A does not have: zeros
+                const uint32_t r0 = 16u * i + r8, c = rank * act_rows + r0;
+                src[i] = r0 < act_rows && c < x.rows ? source_row(p.x, x.row0 + c) : 0xffffffffu;
+            }
+            for (uint32_t l = 0; l < ns; ++l) {
+                if (!warp_wait(step_empty(r.i), r.phase ^ 1u, abort_flag)) { give_up(62, x.expert, l); ok = false; break; }
+                const uint32_t to = at + r.i * act_stride;
+                const uint16_t* from = p.x.a + l * KS + piece * 8u;
 #pragma unroll
-                        for (int h = 0; h < KS / kSlab; ++h) cp_async16_or_zero((i % 2 ? odd : even) + to + h * slab_bytes + i / 2 * 1024u, at + (there ? h * kSlab : 0), there);
-                    }
-                    cp_async_commit();
-                    cp_async_wait_all();
-                    ptx::fence_proxy_async_smem();   // the copies are this thread's writes; tcgen05.mma reads shared memory through the asynchronous proxy
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(step_full(r.i));
-                    r.step(kLoadWarps, kSlots);
+                for (int i = 0; i < kTurns; ++i) {
+                    if (16u * i >= act_rows) break;
+                    const bool there = src[i] < p.x.a_rows;
+                    const uint16_t* row = there ? from + (size_t)src[i] * p.x.lda : p.x.a;
+#pragma unroll
+                    for (int h = 0; h < KS / kSlab; ++h) cp_async16_or_zero(to + h * slab_bytes + i * 2048u, row + (there ? h * kSlab : 0), there);
                 }
-                before += ns;
+                cp_async_commit();
+                issued |= 1u << r.i; parity = (parity & ~(1u << r.i)) | (r.phase << r.i);
+                r.step(1, kSlots);
+                if (++pending > kLag) { cp_async_wait_but<kLag>(); report(); }
             }
-            // not while a commit of rank 0 may still arrive here: the last use of each slot, whoever's it was
-            for (uint32_t s = 0; who == 0 && ok && s < kSlots && s < before; ++s) (void)warp_wait(step_empty(s), (before - 1 - s) / kSlots & 1u, abort_flag);
-        } else {
-            // A lane copies 16 bytes of rows 16 * i + 4 * (which loader) + lane / 8 of this CTA's half, per 64 k.
-            const uint32_t r8 = (uint32_t)(warp - kFirstLoad) * 4 + ((uint32_t)lane >> 3), piece = (uint32_t)lane & 7u;
-            const uint32_t at = smem_base + off_act + r8 * 128u + ((piece ^ (r8 & 7u)) << 4);   // 16 rows on: the same place in the swizzle
-            Ring r{0, 0}, rp{0, 0};       // of the step that comes next, of the oldest one that has not been reported
-            uint32_t pending = 0, issued = 0, parity = 0;
-            bool ok = true;
-            // The copies are this thread's writes; tcgen05.mma reads shared memory through the asynchronous proxy.
-            auto report = [&] {
-                ptx::fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(step_full(rp.i));
-                rp.step(1, kSlots);
-                --pending;
-            };
-            while (ok && next(x)) {
-                const uint32_t act_rows = x.height / 2, slab_bytes = act_rows * 128u;   // act_rows: a multiple of 16
-                uint32_t src[8];
-    #pragma unroll
-                for (int i = 0; i < 8; ++i) {   // rows behind the last one, and those that A does not have: zeros
-                    const uint32_t r0 = 16u * i + r8, c = rank * act_rows + r0;
-                    src[i] = r0 < act_rows && c < x.rows ? source_row(p.x, x.row0 + c) : 0xffffffffu;
-                }
-                for (uint32_t l = 0; l < ns; ++l) {
-                    // a free slot: go on; otherwise first report all that is under way
-                    if (!__all_sync(0xffffffffu, ptx::mbar_test_wait(step_empty(r.i), r.phase ^ 1u))) {
-                        if (pending) { cp_async_wait_all(); while (pending) report(); }
-                        if (!warp_wait(step_empty(r.i), r.phase ^ 1u, abort_flag)) { give_up(62, x.expert, l); ok = false; break; }
-                    }
-                    const uint32_t to = at + r.i * act_stride;
-                    const uint16_t* from = p.x.a + l * KS + piece * 8u;
-    #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if (16u * i >= act_rows) break;
-                        const bool there = src[i] < p.x.a_rows;
-                        const uint16_t* row = there ? from + (size_t)src[i] * p.x.lda : p.x.a;
-    #pragma unroll
-                        for (int h = 0; h < KS / kSlab; ++h) cp_async16_or_zero(to + h * slab_bytes + i * 2048u, row + (there ? h * kSlab : 0), there);
-                    }
-                    cp_async_commit();
-                    ++pending;
-                    issued |= 1u << r.i; parity = (parity & ~(1u << r.i)) | (r.phase << r.i);
-                    r.step(1, kSlots);
-                    if (pending > 2) { cp_async_wait_but2(); report(); }
-                }
-            }
-            cp_async_wait_all();
-            while (pending) report();
-            for (uint32_t s = 0; s < kSlots; ++s)   // not while a commit of rank 0 may still arrive here
-                if (issued & (1u << s)) (void)warp_wait(step_empty(s), (parity >> s) & 1u, abort_flag);
         }
+        cp_async_wait_but<0>();
+        while (pending) report();
+        for (uint32_t s = 0; s < kSlots; ++s)   // not while a commit of rank 0 may still arrive here
+            if (issued & (1u << s)) (void)warp_wait(step_empty(s), (parity >> s) & 1u, abort_flag);
     } else {
         // ======================= epilogue =======================
         ptx::regs_up<regs_epi(CG)>();
