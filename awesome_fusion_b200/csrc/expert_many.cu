@@ -434,7 +434,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
         // twice: with kSlots - kLag steps the tensor cores have enough.  (Each step waited for as soon as the next slot was not free yet: 1000 cycles a step,
         // whatever its height.)  A lane copies 16 bytes of rows 16 * i + 4 * (which loader) + lane / 8 of this CTA's half, per 64 k.
         ptx::regs_down<kRegsLoad>();
-        constexpr uint32_t kLag = kSlots / 2 - 1;
+        constexpr uint32_t kLag = LOW ? 3 : kSlots / 2 - 1;
         const uint32_t r8 = (uint32_t)(warp - kFirstLoad) * 4 + ((uint32_t)lane >> 3), piece = (uint32_t)lane & 7u;
         const uint32_t at = smem_base + off_act + r8 * 128u + ((piece ^ (r8 & 7u)) << 4);   // 16 rows on: the same place in the swizzle
         Ring r{0, 0}, rp{0, 0};       // of the step that comes next, of the oldest one that has not been reported
