@@ -89,7 +89,7 @@ __device__ __forceinline__ uint32_t source_row(const ExpertParams& p, uint32_t r
 }
 
 // v / (1 + exp(-v)) for a result that is rounded to bf16: the product -v log2(e) is rounded once, so the exponential is off by |v| 2^-24 and a little (2^-17 at
-// |v| = 87, where it leaves fp32), a 500th of the rounding to come.  (sigmoid() of activation.cuh has three times the instructions: the drain of an accumulator of 256
+// |v| = 87, where it leaves fp32), a 500th of the rounding to come.  (sigmoid() of pair.cu has three times the instructions: the drain of an accumulator of 256
 // gated columns waits for them.)  Below -128 infinity gives -0, at -infinity NaN, as the quotient would.
 __device__ __forceinline__ float silu(float v) {
     float e, r;

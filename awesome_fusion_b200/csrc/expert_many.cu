@@ -6,7 +6,8 @@
 // one tcgen05.mma.cta_group::2 reads both halves.  An expert's rows are cut into strips of equal height, a multiple of 32.
 //
 //   warp 0        TMA: raw weight blocks, 128 channels x 128 bytes, 128-byte swizzle
-//   warp 2        rank 0: tcgen05.mma 256 x height x 16;  rank 1: reports to rank 0 that its half of a step is complete
+//   warp 2        rank 0: tcgen05.mma 256 x height x 16 (low strips: with warp 3, every second step each, into an accumulator each);  rank 1: reports
+//                 to rank 0 that its half of a step is complete
 //   warps 4-11    epilogue, two per lane quarter: accumulator -> registers -> (accumulator free) -> shared memory -> C
 //   then          converters: CG groups of four warps; group g takes every CG-th step of k (KS = 128 or 64 wide)
 //   last four     the rows of A: 16-byte copies to shared memory, written in the 128-byte swizzle.  (A TMA gather of four rows takes 65 cycles of
@@ -21,6 +22,11 @@
 // 1650 cycles per step of 128 rows, the chain from accumulator to registers and back; 2048 tokens, 64 experts of 2048 x 4096 int4: 516 us.)
 //
 // Every role walks the same tiles (ExpertTable): worker, worker + workers, ...
+//
+// What bounds it.  Strips of 256 rows: the tensor pipe, under the power limit (8192 rows on 8 experts of 22016 x 4096 int8, gated: 1106 us = 1.34 PFLOP/s; 1054 cycles per
+// step of 128 k where the instructions take 1000), and per tile the drain of the only accumulator (2000 to 3000 cycles).  Lower ones: the hand-offs, 1000 cycles
+// per step down to 130 rows (16384 rows on 64 experts of 2048 x 4096 int4 group-128: 302 us), 900 up to 64 (1024 rows: 122 us; the converters of int4 in groups
+// need 2600 cycles for a step, four of them at a time; int8 per channel 109 us, 4.9 TB/s of weights).
 #include <cuda_fp16.h>
 #include "dequant.cuh"
 #include "expert_common.cuh"

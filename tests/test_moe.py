@@ -109,6 +109,28 @@ def test_combine_refuses(lib, changes):
     assert _combine(lib, **changes) == E_BAD
 
 
+def test_torch_operators_infer_shapes_and_have_no_cpu_path():
+    import awesome_fusion_b200.torch_op  # noqa: F401
+    ops, meta = torch.ops.afb, dict(device="meta")
+    weights, ids, offsets, row_pair, pair_row = ops.moe_route(torch.empty((5, 16), **meta), 3, True)
+    assert [t.shape for t in (weights, ids, offsets, row_pair, pair_row)] == [(5, 3), (5, 3), (17,), (15,), (5, 3)]
+    assert weights.dtype == torch.float32 and {t.dtype for t in (ids, offsets, row_pair, pair_row)} == {torch.int32}
+    a, b, scale = torch.empty((5, 256), dtype=torch.bfloat16, **meta), torch.empty((16, 64, 128), dtype=torch.uint8, **meta), torch.empty((16, 64, 2), dtype=torch.bfloat16, **meta)
+    assert ops.expert_gemm(a, b, scale, None, offsets, row_pair, 3, 4, 128, False, False, True).shape == (15, 32)
+    assert ops.expert_gemm(a, b, scale, None, offsets, None, 1, 4, 128, False).shape == (5, 64)
+    assert ops.moe_combine(torch.empty((15, 64), dtype=torch.bfloat16, **meta), weights, pair_row).shape == (5, 64)
+    for bad in ((a, b, scale[:, :, :1], None, offsets, None, 1, 4, 128, False), (a, b, scale, None, offsets, None, 2, 4, 128, False), (a, b, scale, None, offsets[:5], None, 1, 4, 128, False)):
+        with pytest.raises(Exception):
+            ops.expert_gemm(*bad)
+    for bad in ((torch.empty((5, 16), **meta), 17, True), (torch.empty((5, 16), **meta), 0, True), (torch.empty((5, 1025), **meta), 2, True)):
+        with pytest.raises(Exception):
+            ops.moe_route(*bad)
+    with pytest.raises(Exception):
+        ops.moe_route(torch.zeros((2, 4)), 1, True)
+    with pytest.raises(Exception):
+        ops.moe_combine(torch.zeros((2, 8), dtype=torch.bfloat16), torch.zeros((1, 2)), torch.zeros((1, 2), dtype=torch.int32))
+
+
 # ---- plain forms in 64 bits -------------------------------------------------------------------------------------------------------------------
 
 def plain_route(logits, top_k, renormalize):
