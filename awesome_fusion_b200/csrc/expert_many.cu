@@ -37,7 +37,7 @@ namespace {
 
 constexpr int kFirstEpi = 4, kEpiWarps = 8, kFirstConv = kFirstEpi + kEpiWarps, kLoadWarps = 4;
 // CG groups of converters: four where strips are low and a group's chain (wait, load, unpack, tcgen05.st, arrive: 1800 cycles) is what a step waits for, two where
-// they are high and more warps only get in each other's way (1024 rows on 64 experts of 2048 x 4096 int4: 141 us with four, 153 with two; 16384 rows: 340, 320).
+// they are high and more warps only get in each other's way (1024 rows on 64 experts of 2048 x 4096 int4: 141 us with four, 153 with two; 16384 rows, before the copies of the rows were reported late: 340, 320).
 __host__ __device__ constexpr int many_threads(int cg) { return 32 * (kFirstConv + 4 * cg + kLoadWarps); }        // 1024 or 768: launched with 64 or 80 registers a thread
 constexpr uint32_t kRegsCtrl = 40, kRegsLoad = 40;
 __host__ __device__ constexpr uint32_t regs_epi(int cg) { return cg == 4 ? 104 : 136; }
