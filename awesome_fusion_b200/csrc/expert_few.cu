@@ -17,7 +17,7 @@
 //
 // What bounds it.  int8 per channel: HBM (32 rows on 8 experts of 22016 x 4096, gated: 114 to 140 us with the experts' shares of the rows, 5.2 to 6.3 TB/s).  int4 in groups:
 // instructions, 650 to 780 per warp and stage of 4 KB, four warps a scheduler at 0.55 of the issue slots (8 rows on 8 experts of 2048 x 4096: 14 us, 2.4 TB/s
-// from L2; 16 rows each on 64 experts: 137 us, where the form for many rows takes 122).
+// from L2; 16 rows each on 64 experts: 137 us, where the form for many rows takes 119).
 #include "dequant.cuh"
 #include "decode_common.cuh"
 #include "expert_common.cuh"

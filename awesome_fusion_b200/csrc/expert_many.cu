@@ -25,7 +25,7 @@
 //
 // What bounds it.  Strips of 256 rows: the tensor pipe, under the power limit (8192 rows on 8 experts of 22016 x 4096 int8, gated: 1106 us = 1.34 PFLOP/s; 1054 cycles per
 // step of 128 k where the instructions take 1000), and per tile the drain of the only accumulator (2000 to 3000 cycles).  Lower ones: the hand-offs, 1000 cycles
-// per step down to 130 rows (16384 rows on 64 experts of 2048 x 4096 int4 group-128: 302 us), 900 up to 64 (1024 rows: 122 us; the converters of int4 in groups
+// per step down to 130 rows (16384 rows on 64 experts of 2048 x 4096 int4 group-128: 302 us), 870 up to 64 (1024 rows: 119 us; the converters of int4 in groups
 // need 2600 cycles for a step, four of them at a time; int8 per channel 109 us, 4.9 TB/s of weights).
 #include <cuda_fp16.h>
 #include "dequant.cuh"
@@ -36,14 +36,18 @@ namespace afb {
 namespace {
 
 constexpr int kFirstEpi = 4, kEpiWarps = 8, kFirstConv = kFirstEpi + kEpiWarps, kLoadWarps = 4;
-// CG groups of converters: four where strips are low and a group's chain (wait, load, unpack, tcgen05.st, arrive: 1800 cycles) is what a step waits for, two where
+// CG groups of converters: four where strips are low and a group's chain (wait, load, unpack, tcgen05.st, arrive) is what a step waits for, two where
 // they are high and more warps only get in each other's way (1024 rows on 64 experts of 2048 x 4096 int4: 141 us with four, 153 with two; 16384 rows, before the copies of the rows were reported late: 340, 320).
 __host__ __device__ constexpr int many_threads(int cg) { return 32 * (kFirstConv + 4 * cg + kLoadWarps); }        // 1024 or 768: launched with 64 or 80 registers a thread
-constexpr uint32_t kRegsCtrl = 40, kRegsLoad = 40;
-__host__ __device__ constexpr uint32_t regs_epi(int cg) { return cg == 4 ? 104 : 136; }
-__host__ __device__ constexpr uint32_t regs_conv(int cg) { return cg == 4 ? 56 : 64; }
-__host__ __device__ constexpr uint32_t regs_all(int cg) { return 128 * kRegsCtrl + 32 * kEpiWarps * regs_epi(cg) + 128 * cg * regs_conv(cg) + 32 * kLoadWarps * kRegsLoad; }
-static_assert(regs_all(2) <= 80u * many_threads(2) && regs_all(4) <= 64u * many_threads(4), "shares of the registers");
+// Registers a thread of each role.  HEAVY: converters of int4 in groups, which hold the words, the scales and the results of a step; with 56 they go to
+// local memory and back 13 times a step (1024 rows: 123 us; with 64: 119; int8 per channel, which needs no more than 56, 109 and 111).
+struct Shares { uint32_t ctrl, epi, conv, load; };
+__host__ __device__ constexpr Shares shares(int cg, bool heavy) { return cg == 2 ? Shares{40, 136, 64, 40} : heavy ? Shares{32, 96, 64, 32} : Shares{40, 104, 56, 40}; }
+__host__ __device__ constexpr uint32_t regs_all(int cg, bool heavy) {
+    const Shares r = shares(cg, heavy);
+    return 128 * r.ctrl + 32 * kEpiWarps * r.epi + 128 * cg * r.conv + 32 * kLoadWarps * r.load;
+}
+static_assert(regs_all(2, false) <= 80u * many_threads(2) && regs_all(4, false) <= 64u * many_threads(4) && regs_all(4, true) <= 64u * many_threads(4), "shares of the registers");
 constexpr int kMaxRaw = 12, kMaxSlots = 8, kMaxAcc = 2;
 __host__ __device__ constexpr uint32_t slots(int ks, bool low) { return ks == 128 && !low ? 4 : 6; }   // steps under way, in 256 columns at most (low strips: 384)
 constexpr uint32_t kTmemCols = 512;
@@ -194,6 +198,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
     constexpr uint32_t SPB = (BITS == 8 ? 128 : 256) / KS;   // steps per raw block
     constexpr uint32_t kSlotCols = KS / 2;                   // TMEM columns of a step's weights
     constexpr uint32_t kSlots = slots(KS, LOW);
+    constexpr Shares kShares = shares(CG, BITS == 4 && GROUPED);
     constexpr int kConvGroups = CG, kFirstLoad = kFirstConv + 4 * CG;
     constexpr uint32_t kIssuers = LOW ? 2 : 1;
     static_assert(!LOW || (CG == 4 && kSlots % 2 == 0), "a slot's steps are one issuer's");
@@ -257,7 +262,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
 
     // Warps 0 to 3 run their loops as whole warps and elect a lane for the asynchronous instructions only (stream.cu).
     if (warp < kFirstEpi) {
-        ptx::regs_down<kRegsCtrl>();
+        ptx::regs_down<kShares.ctrl>();
         Ring r{0, 0};
         uint32_t issued = 0, parity = 0;
         bool ok = true;
@@ -322,7 +327,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
         }
     } else if (warp >= kFirstConv && warp < kFirstLoad) {
         // ======================= converters =======================
-        ptx::regs_down<regs_conv(CG)>();
+        ptx::regs_down<kShares.conv>();
         const uint32_t g = (uint32_t)(warp - kFirstConv) >> 2, quarter = (uint32_t)warp & 3u;
         const uint32_t ch = quarter * 32 + lane;
         const uint32_t flip = BITS == 8 ? flip8(p.x.enc) : flip4(p.x.enc);
@@ -439,7 +444,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
         // All four warps copy a step together and report it when they have issued kLag more, so that neither a copy's latency nor a slot's is waited for
         // twice: with kSlots - kLag steps the tensor cores have enough.  (Each step waited for as soon as the next slot was not free yet: 1000 cycles a step,
         // whatever its height.)  A lane copies 16 bytes of rows 16 * i + 4 * (which loader) + lane / 8 of this CTA's half, per 64 k.
-        ptx::regs_down<kRegsLoad>();
+        ptx::regs_down<kShares.load>();
         constexpr uint32_t kLag = LOW ? 3 : kSlots / 2 - 1;
         const uint32_t r8 = (uint32_t)(warp - kFirstLoad) * 4 + ((uint32_t)lane >> 3), piece = (uint32_t)lane & 7u;
         const uint32_t at = smem_base + off_act + r8 * 128u + ((piece ^ (r8 & 7u)) << 4);   // 16 rows on: the same place in the swizzle
@@ -487,7 +492,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
             if (issued & (1u << s)) (void)warp_wait(step_empty(s), (parity >> s) & 1u, abort_flag);
     } else {
         // ======================= epilogue =======================
-        ptx::regs_up<regs_epi(CG)>();
+        ptx::regs_up<kShares.epi>();
         const uint32_t quarter = (uint32_t)warp & 3u, half = (uint32_t)(warp - kFirstEpi) >> 2, ch = quarter * 32 + lane;
         constexpr int kPacks = LOW ? 2 : 8;   // of 16 columns: this warp's half of a strip
         const bool odd = lane & 1, gated = p.x.gated != 0, act = p.x.silu != 0;
@@ -648,7 +653,7 @@ int launch_groups(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uin
         cudaFuncAttributes attr;
         cudaError_t e = cudaFuncGetAttributes(&attr, kern);
         if (e != cudaSuccess) return cuda_fail(e);
-        if ((uint32_t)(attr.numRegs * many_threads(CG)) < regs_all(CG)) return AFB_ERR_UNSUPPORTED;   // the shares come out of what the block is launched with
+        if ((uint32_t)(attr.numRegs * many_threads(CG)) < regs_all(CG, BITS == 4 && GROUPED)) return AFB_ERR_UNSUPPORTED;   // the shares come out of what the block is launched with
         e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
         if (e != cudaSuccess) return cuda_fail(e);
         attr_set.mark(ctx->device);
