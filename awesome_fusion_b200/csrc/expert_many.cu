@@ -335,6 +335,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
         const Nibbles nib = nibbles(p.x.packed != 0);
         const bool has_zero = p.x.zero != nullptr;
         const uint32_t groups_per_row = GROUPED ? p.x.k >> p.x.group_shift : 0;
+        const bool half_scale = p.x.scale_dtype == AFB_SCALE_BF16, two_groups = GROUPED && p.x.group_shift < 7;
         auto zero_of = [&](size_t i) { return BITS == 8 ? decode_zero8(p.x.zero[i], p.x.enc) : decode_zero4(p.x.zero[i], p.x.enc); };
         // bf16: weight * 2^-6 in one step (dequant.cuh).  fp16: an unsigned weight u, zero-extended, is u * 2^-24; fma makes (u - 128 - zero) * 2^-9 of it,
         // exactly, and a multiplication by the channel's scale, at most 2^15, rounds once.
@@ -346,7 +347,8 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
         uint32_t add[KS / 64];
 #pragma unroll
         for (int h = 0; h < KS / 64; ++h) add[h] = add_of(0);
-        const uint32_t row = p.off_raw + ch * 128, swz = (ch & 7u) << 4, lanes = (quarter * 32u) << 16;
+        const uint32_t row = p.off_raw + ch * 128 + ((ch & 7u) << 4),   // its first 16 bytes in the swizzle; piece i is 16 * i away, by xor
+                       lanes = (quarter * 32u) << 16;
         uint32_t steps_before = 0, blocks_before = 0;   // of the tiles walked so far
         bool ok = true;
         while (ok && next(x)) {
@@ -357,16 +359,19 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                 for (int h = 0; h < KS / 64; ++h) add[h] = add_of(zero_of(chan));
             }
             const float mult = GROUPED ? p.channel_mult[chan] : 1.f;
-            // scales and zero-points of this group's next step, of each 64 k, as they are stored
+            // scales and zero-points of this group's next step, of each 64 k that have their own, as they are stored
+            const char* scales = GROUPED ? reinterpret_cast<const char*>(p.x.scale) + chan * groups_per_row * (half_scale ? 2 : 4) : nullptr;
+            const uint8_t* zeros = GROUPED && has_zero ? p.x.zero + chan * groups_per_row : nullptr;
             uint32_t sc_nxt[KS / 64] = {}, z_nxt[KS / 64] = {};
             auto load_group = [&](uint32_t l) {
                 if constexpr (GROUPED) {
                     if (l >= ns) return;
 #pragma unroll
                     for (int h = 0; h < KS / 64; ++h) {
-                        const size_t i = chan * groups_per_row + ((l * KS + h * 64) >> p.x.group_shift);
-                        sc_nxt[h] = p.x.scale_dtype == AFB_SCALE_BF16 ? reinterpret_cast<const uint16_t*>(p.x.scale)[i] : reinterpret_cast<const uint32_t*>(p.x.scale)[i];
-                        if (has_zero) z_nxt[h] = p.x.zero[i];
+                        if (h && !two_groups) break;
+                        const uint32_t i = (l * KS + h * 64) >> p.x.group_shift;
+                        sc_nxt[h] = half_scale ? reinterpret_cast<const uint16_t*>(scales)[i] : reinterpret_cast<const uint32_t*>(scales)[i];
+                        if (has_zero) z_nxt[h] = zeros[i];
                     }
                 }
             };
@@ -381,7 +386,8 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                 if (GROUPED) {
 #pragma unroll
                     for (int h = 0; h < KS / 64; ++h) {
-                        sc[h] = f16_dup(__uint_as_float(p.x.scale_dtype == AFB_SCALE_BF16 ? sc_nxt[h] << 16 : sc_nxt[h]) * mult);
+                        if (h && !two_groups) { sc[h] = sc[0]; add[h] = add[0]; break; }
+                        sc[h] = f16_dup(__uint_as_float(half_scale ? sc_nxt[h] << 16 : sc_nxt[h]) * mult);
                         if (has_zero) add[h] = add_of(BITS == 8 ? decode_zero8(z_nxt[h], p.x.enc) : decode_zero4(z_nxt[h], p.x.enc));
                     }
                     load_group(l + kConvGroups);
@@ -396,7 +402,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                     uint32_t w[kWords];
 #pragma unroll
                     for (int i = 0; i < kWords / 4; ++i) {
-                        const uint32_t at = raw + ((((sub * kPieces + h) * (kWords / 4) + i) << 4) ^ swz);
+                        const uint32_t at = (raw ^ (sub * (kPieces * kWords * 4))) ^ ((h * (kWords / 4) + i) << 4);
                         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3]) : "r"(at));
                     }
 #pragma unroll
