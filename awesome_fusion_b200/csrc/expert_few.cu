@@ -118,7 +118,7 @@ expert_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const FewParams p)
         uint32_t issued = 0, parity = 0;
         bool ok = true;
         for (uint32_t i = blockIdx.x; ok && i < tiles; i += gridDim.x) {
-            table.tile(x, i, 1, t);
+            table.tile<1>(x, i, t);
             const int y = (int)(t.expert * x.n + t.block * kCh);
             const uint16_t* src[8 * MT / kTurn];   // of this lane's piece of the next stage
             uint32_t size[8 * MT / kTurn];         // bytes that there are of it; the rest is zeros
@@ -170,7 +170,7 @@ expert_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const FewParams p)
         uint32_t before = 0;   // stages of the tiles walked so far
         bool ok = true;
         for (uint32_t i = blockIdx.x; i < tiles; i += gridDim.x) {
-            table.tile(x, i, 1, t);
+            table.tile<1>(x, i, t);
             const uint32_t n0 = t.block * kCh;
             const bool two = MT > 1 && t.rows > 8;   // eight rows or less take one instruction where there could be two
             uint32_t chan[4];      // rows of B of this lane's channels: 8 apart
@@ -400,7 +400,7 @@ int launch_rows(const CUtensorMap& tw, const FewParams& p, uint32_t bits, uint32
 int launch_expert_few(const ExpertParams& q, uint32_t bits, uint32_t group, DeviceCtx* ctx, cudaStream_t s) {
     FewParams p{};
     p.x = q;
-    p.x.n_blocks = (q.n + kCh - 1) / kCh;
+    p.x.set_blocks((q.n + kCh - 1) / kCh);
     p.stages_per_tile = (uint32_t)(((uint64_t)q.k * bits / 8 + 127) / 128);
     p.c_vec = q.ldc % 4 == 0 && (uintptr_t)q.c % 8 == 0;
     p.status = ctx->status;

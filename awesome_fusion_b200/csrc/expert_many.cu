@@ -252,7 +252,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
     uint32_t t = worker;   // every role of both CTAs walks the same list of tiles
     auto next = [&](Strip& s) {
         if (t >= tiles) return false;
-        table.tile(p.x, t, kUnit, s);
+        table.tile<kUnit>(p.x, t, s);
         s.n0 = (2 * s.block + rank) * kCh;
         t += workers;
         return true;
@@ -690,7 +690,7 @@ int launch_expert_many(const ExpertParams& q, uint32_t bits, uint32_t group, Dev
     ManyParams p{};
     p.x = q;
     const uint32_t ks = q.k % 128 == 0 ? 128 : 64, spb = (bits == 8 ? 128 : 256) / ks;
-    p.x.n_blocks = (q.n + 2 * kCh - 1) / (2 * kCh);
+    p.x.set_blocks((q.n + 2 * kCh - 1) / (2 * kCh));
     p.steps = q.k / ks;
     const uint32_t per_block = p.steps % spb == 0 ? spb : 1;
     // Up to 128 rows there are two accumulators, and twice the raw blocks under way.  Up to 64 each of two issuers has one, in return for six slots (four, and two
