@@ -100,6 +100,11 @@ struct ExpertTable {
     }
 };
 
+// Arrives on `bar` when this thread's copies so far are complete.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 // Row of A behind row r of C; a value outside [0, a_rows): none, reads as zeros.
 __device__ __forceinline__ uint32_t source_row(const ExpertParams& p, uint32_t r) {
     if (!p.row_pair) return r;

@@ -53,10 +53,6 @@ __device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint3
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-// Arrives on `bar` when this thread's copies so far are complete.
-__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
 // The unpack's addend for a zero-point byte: -(the byte as an unsigned weight) * 2^-6, by the unpack's own multiply-add.
 template <int BITS> __device__ __forceinline__ uint32_t zero_addend(uint32_t zbyte, uint32_t flip) {
     const uint32_t u = (zbyte ^ flip) & (BITS == 8 ? 0xffu : 0xfu);

@@ -73,8 +73,7 @@ struct ManyParams {
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <uint32_t N> __device__ __forceinline__ void cp_async_wait_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }   // all but the newest N
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // Two fp16 values at a time.
 __device__ __forceinline__ uint32_t f16x2_mul(uint32_t a, uint32_t b) {
@@ -223,7 +222,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
 
     if (warp == 0 && lane == 0) {
         for (uint32_t s = 0; s < p.raw_stages; ++s) { ptx::mbar_init(raw_full(s), 1); ptx::mbar_init(raw_empty(s), 4 * SPB); }
-        for (uint32_t s = 0; s < kSlots; ++s) { ptx::mbar_init(step_full(s), 4 + kLoadWarps + (rank == 0 ? 1 : 0)); ptx::mbar_init(step_empty(s), 1); }
+        for (uint32_t s = 0; s < kSlots; ++s) { ptx::mbar_init(step_full(s), 4 + 32 * kLoadWarps + (rank == 0 ? 1 : 0)); ptx::mbar_init(step_empty(s), 1); }
         for (uint32_t s = 0; s < (LOW ? 2u : p.accs); ++s) { ptx::mbar_init(acc_full(s), 1); ptx::mbar_init(acc_empty(s), 2 * kEpiWarps); }
         *abort_flag = 0;
         ptx::fence_mbar_init();
@@ -297,6 +296,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                 if (!warp_wait(acc_empty(acc), rc.phase ^ 1u, abort_flag)) { give_up(63, x.expert, 0); break; }
                 for (; g < before + ns; g += kIssuers) {
                     if (!__all_sync(0xffffffffu, ready) && !warp_wait(step_full(r.i), r.phase, abort_flag)) { give_up(64, x.expert, g); ok = false; break; }
+                    ptx::fence_proxy_async_smem();
                     ptx::tc_fence_after_sync();
                     const uint32_t ta = slot_base + r.i * kSlotCols, done = step_empty(r.i);
                     const uint64_t db = desc0 + r.i * (act_stride >> 4);
@@ -318,6 +318,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
             while (ok && next(x)) {
                 for (uint32_t l = 0; l < ns; ++l) {
                     if (!warp_wait(step_full(r.i), r.phase, abort_flag)) { give_up(65, x.expert, l); ok = false; break; }
+                    ptx::fence_proxy_async_smem();
                     ptx::tc_fence_after_sync();
                     ptx::tc_fence_before_sync();
                     if (ptx::elect_one()) ptx::mbar_arrive_remote(step_full(r.i), 0);
@@ -447,27 +448,22 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
         }
     } else if (warp >= kFirstLoad) {
         // ======================= rows of A =======================
-        // All four warps copy a step together and report it when they have issued kLag more, so that neither a copy's latency nor a slot's is waited for
-        // twice: with kSlots - kLag steps the tensor cores have enough.  (Each step waited for as soon as the next slot was not free yet: 1000 cycles a step,
-        // whatever its height.)  A lane copies 16 bytes of rows 16 * i + 4 * (which loader) + lane / 8 of this CTA's half, per 64 k.
+        // All four warps copy a step together.  The copies report themselves when they are complete, so the warps run ahead as far as there are slots.  They are these
+        // threads' writes, and tcgen05.mma reads shared memory through the asynchronous proxy: the issuers (rank 1: the reporter) fence between the two once they
+        // have waited.  (Waited for and reported by the warps, one to three steps later: 16384 rows on 64 experts of int4 299 us, 8192 rows of int8 1128; now 287 and
+        // 1072.)  A lane copies 16 bytes of rows 16 * i + 4 * (which loader) + lane / 8 of this CTA's half, per 64 k.
         ptx::regs_down<kShares.load>();
-        constexpr uint32_t kLag = LOW ? 3 : kSlots / 2 - 1;
         const uint32_t r8 = (uint32_t)(warp - kFirstLoad) * 4 + ((uint32_t)lane >> 3), piece = (uint32_t)lane & 7u;
         const uint32_t at = smem_base + off_act + r8 * 128u + ((piece ^ (r8 & 7u)) << 4);   // 16 rows on: the same place in the swizzle
-        Ring r{0, 0}, rp{0, 0};       // of the step that comes next, of the oldest one that has not been reported
-        uint32_t pending = 0, issued = 0, parity = 0;
+        Ring r{0, 0};
+        uint32_t issued = 0, parity = 0;
         bool ok = true;
-        // The copies are this thread's writes; tcgen05.mma reads shared memory through the asynchronous proxy.
-        auto report = [&] {
-            ptx::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(step_full(rp.i));
-            rp.step(1, kSlots);
-            --pending;
-        };
         while (ok && next(x)) {
             const uint32_t act_rows = x.height / 2, slab_bytes = act_rows * 128u;   // act_rows: a multiple of 16
             constexpr int kTurns = LOW ? 2 : 8;
+            // Low strips leave out what is behind the last row: the columns of D of those rows are never stored.  (High ones, whose last is not much lower, lose 2 to
+            // 4 % to the test.)
+            const uint32_t to_copy = !LOW ? act_rows : x.rows > rank * act_rows ? min(act_rows, x.rows - rank * act_rows) : 0u;
             uint32_t src[kTurns];
 #pragma unroll
             for (int i = 0; i < kTurns; ++i) {   // rows behind the last one, and those that A does not have: zeros
@@ -480,20 +476,18 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                 const uint16_t* from = p.x.a + l * KS + piece * 8u;
 #pragma unroll
                 for (int i = 0; i < kTurns; ++i) {
-                    if (16u * i >= act_rows) break;
+                    if (16u * i >= to_copy) break;
                     const bool there = src[i] < p.x.a_rows;
                     const uint16_t* row = there ? from + (size_t)src[i] * p.x.lda : p.x.a;
 #pragma unroll
                     for (int h = 0; h < KS / kSlab; ++h) cp_async16_or_zero(to + h * slab_bytes + i * 2048u, row + (there ? h * kSlab : 0), there);
                 }
-                cp_async_commit();
+                cp_async_arrive(step_full(r.i));
                 issued |= 1u << r.i; parity = (parity & ~(1u << r.i)) | (r.phase << r.i);
                 r.step(1, kSlots);
-                if (++pending > kLag) { cp_async_wait_but<kLag>(); report(); }
             }
         }
-        cp_async_wait_but<0>();
-        while (pending) report();
+        cp_async_wait_all();   // never leave with a copy still writing this CTA's shared memory
         for (uint32_t s = 0; s < kSlots; ++s)   // not while a commit of rank 0 may still arrive here
             if (issued & (1u << s)) (void)warp_wait(step_empty(s), (parity >> s) & 1u, abort_flag);
     } else {
