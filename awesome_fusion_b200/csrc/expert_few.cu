@@ -17,7 +17,7 @@
 //
 // What bounds it.  int8 per channel: HBM (32 rows on 8 experts of 22016 x 4096, gated: 114 to 140 us with the experts' shares of the rows, 5.2 to 6.3 TB/s).  int4 in groups:
 // instructions, 650 to 780 per warp and stage of 4 KB, four warps a scheduler at 0.55 of the issue slots (8 rows on 8 experts of 2048 x 4096: 14 us, 2.4 TB/s
-// from L2; 16 rows each on 64 experts: 137 us, where the form for many rows takes 119).
+// from L2; 16 rows each on 64 experts: 137 us, where the form for many rows takes 114).
 #include "dequant.cuh"
 #include "decode_common.cuh"
 #include "expert_common.cuh"
@@ -447,9 +447,9 @@ extern "C" int afb_expert_gemm_launch(const afb_expert_gemm_args* x, void* strea
     for (uint32_t g = a.group_size; g > 1; g >>= 1) ++p.group_shift;
     p.gated = x->gated; p.silu = x->activation == AFB_ACT_SILU ? 1u : 0u;
     // Which form is the faster one, by the mean of the rows per expert (us, few / many; their own numbers of rows spread around it):
-    //   64 experts of 2048 x 4096 gated, int4 group-128: 8 rows 90 / 105, 12: 116 / 122, 16: 137 / 121, 24: 170 / 136;  int8: 4: 84 / 82, 8: 105 / 92
-    //   8 of 11008 x 4096, int4 group-128: 12: 78 / 89, 16: 92 / 91, 24: 125 / 91;  int8: 4: 84 / 80, 12: 90 / 81
-    //   16 of 4096 x 2816, int4 group-64: 8: 51 / 58, 12: 61 / 58, 24: 84 / 60;  128 of 1536 x 2048, int8 group-128: 4: 76 / 81, 8: 96 / 89
+    //   64 experts of 2048 x 4096 gated, int4 group-128: 8 rows 86 / 97, 12: 110 / 112, 16: 133 / 112, 24: 165 / 126;  int8: 4: 82 / 80, 8: 102 / 92
+    //   8 of 11008 x 4096, int4 group-128: 12: 74 / 85, 16: 88 / 85, 24: 121 / 85;  int8: 4: 82 / 80, 12: 88 / 80
+    //   16 of 4096 x 2816, int4 group-64: 8: 50 / 54, 12: 59 / 54, 24: 80 / 56;  128 of 1536 x 2048, int8 group-128: 4: 72 / 81, 8: 92 / 87
     const bool many = a.variant == AFB_VARIANT_PREFILL || (a.variant == AFB_VARIANT_AUTO && (uint64_t)a.m > (a.b_bits == 8 ? 4ull : 12ull) * x->experts);
     if (many) {
         bool done = false;

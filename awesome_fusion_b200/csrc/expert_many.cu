@@ -9,7 +9,7 @@
 //   warp 2        rank 0: tcgen05.mma 256 x height x 16 (low strips: with warp 3, every second step each, into an accumulator each);  rank 1: reports
 //                 to rank 0 that its half of a step is complete
 //   warps 4-11    epilogue, two per lane quarter: accumulator -> registers -> (accumulator free) -> shared memory -> C
-//   then          converters: CG groups of four warps; group g takes every CG-th step of k (KS = 128 or 64 wide)
+//   then          converters: four groups of four warps; group g takes every fourth step of k (KS = 128 or 64 wide)
 //   last four     the rows of A: 16-byte copies to shared memory, written in the 128-byte swizzle.  (A TMA gather of four rows takes 65 cycles of
 //                 the issuing warp, which has to make every lane's row numbers uniform first: 4200 cycles per step of 256 rows.)
 //
@@ -23,10 +23,10 @@
 //
 // Every role walks the same tiles (ExpertTable): worker, worker + workers, ...
 //
-// What bounds it.  Strips of 256 rows: the tensor pipe, under the power limit (8192 rows on 8 experts of 22016 x 4096 int8, gated: 1106 us = 1.34 PFLOP/s; 1054 cycles per
-// step of 128 k where the instructions take 1000), and per tile the drain of the only accumulator (2000 to 3000 cycles).  Lower ones: the hand-offs, 1000 cycles
-// per step down to 130 rows (16384 rows on 64 experts of 2048 x 4096 int4 group-128: 302 us), 870 up to 64 (1024 rows: 119 us; the converters of int4 in groups
-// need 2600 cycles for a step, four of them at a time; int8 per channel 109 us, 4.9 TB/s of weights).
+// What bounds it.  Strips of 256 rows: the tensor pipe, under the power limit (8192 rows on 8 experts of 22016 x 4096 int8, gated: 1047 us = 1.41 PFLOP/s), and per tile
+// the drain of the only accumulator (2000 to 3000 cycles); where they are lower than that the hand-offs (16384 rows on 64 experts of 2048 x 4096 int4 group-128: 274 us
+// = 1.0 PFLOP/s).  Strips up to 64: int4 in groups by instructions, 0.69 of the issue slots (1024 rows: 114 us; a group of converters needs 2600 cycles for a
+// step, four of them at a time); int8 per channel by HBM (103 us, 5.2 TB/s of weights).
 #include <cuda_fp16.h>
 #include "dequant.cuh"
 #include "expert_common.cuh"
@@ -36,18 +36,19 @@ namespace afb {
 namespace {
 
 constexpr int kFirstEpi = 4, kEpiWarps = 8, kFirstConv = kFirstEpi + kEpiWarps, kLoadWarps = 4;
-// CG groups of converters: four where strips are low and a group's chain (wait, load, unpack, tcgen05.st, arrive) is what a step waits for, two where
-// they are high and more warps only get in each other's way (1024 rows on 64 experts of 2048 x 4096 int4: 141 us with four, 153 with two; 16384 rows, before the copies of the rows were reported late: 340, 320).
-__host__ __device__ constexpr int many_threads(int cg) { return 32 * (kFirstConv + 4 * cg + kLoadWarps); }        // 1024 or 768: launched with 64 or 80 registers a thread
+// Groups of converters.  Four: a group's chain (wait, load, unpack, tcgen05.st, arrive) is what a step waits for where strips are low (1024 rows on 64 experts of
+// 2048 x 4096 int4: 141 us with four, 153 with two), and int4 in groups where they are high (16384 rows: 273 with four, 284 with two); int8 does not mind (8192 rows on 8
+// experts: 1056, 1062).  Six, with four other warps less: slower, the rows of A then come from one warp (1024 rows: 134 where four groups take 115).
+constexpr int kConvGroups = 4, kFirstLoad = kFirstConv + 4 * kConvGroups, kManyThreads = 32 * (kFirstLoad + kLoadWarps);   // 1024: launched with 64 registers a thread
 // Registers a thread of each role.  HEAVY: converters of int4 in groups, which hold the words, the scales and the results of a step; with 56 they go to
 // local memory and back 13 times a step (1024 rows: 123 us; with 64: 119; int8 per channel, which needs no more than 56, 109 and 111).
 struct Shares { uint32_t ctrl, epi, conv, load; };
-__host__ __device__ constexpr Shares shares(int cg, bool heavy) { return cg == 2 ? Shares{40, 136, 64, 40} : heavy ? Shares{32, 96, 64, 32} : Shares{40, 104, 56, 40}; }
-__host__ __device__ constexpr uint32_t regs_all(int cg, bool heavy) {
-    const Shares r = shares(cg, heavy);
-    return 128 * r.ctrl + 32 * kEpiWarps * r.epi + 128 * cg * r.conv + 32 * kLoadWarps * r.load;
+__host__ __device__ constexpr Shares shares(bool heavy) { return heavy ? Shares{32, 96, 64, 32} : Shares{40, 104, 56, 40}; }
+__host__ __device__ constexpr uint32_t regs_all(bool heavy) {
+    const Shares r = shares(heavy);
+    return 128 * r.ctrl + 32 * kEpiWarps * r.epi + 128 * kConvGroups * r.conv + 32 * kLoadWarps * r.load;
 }
-static_assert(regs_all(2, false) <= 80u * many_threads(2) && regs_all(4, false) <= 64u * many_threads(4) && regs_all(4, true) <= 64u * many_threads(4), "shares of the registers");
+static_assert(regs_all(false) <= 64u * kManyThreads && regs_all(true) <= 64u * kManyThreads, "shares of the registers");
 constexpr int kMaxRaw = 12, kMaxSlots = 8, kMaxAcc = 2;
 __host__ __device__ constexpr uint32_t slots(int ks, bool low) { return ks == 128 && !low ? 4 : 6; }   // steps under way, in 256 columns at most (low strips: 384)
 constexpr uint32_t kTmemCols = 512;
@@ -61,7 +62,7 @@ constexpr uint32_t kUnit = 32;           // rows: 16 per epilogue warp
 struct ManyParams {
     ExpertParams x;
     uint32_t steps;           // along K
-    uint32_t raw_stages, accs;
+    uint32_t raw_stages;
     uint32_t slot_first;      // converters wait for their slot before they wait for their raw block
     uint32_t off_raw;         // behind the table
     uint32_t c_vec;           // 16-byte stores of C
@@ -191,16 +192,15 @@ __global__ void __launch_bounds__(kPrepareThreads) expert_prepare_kernel(const P
 
 struct Strip : ExpertStrip { uint32_t n0; };   // n0: of this CTA's 128 channels
 
-template <int BITS, bool GROUPED, int KS, int CG, bool LOW>
-__global__ void __launch_bounds__(many_threads(CG), 1)
+template <int BITS, bool GROUPED, int KS, bool LOW>
+__global__ void __launch_bounds__(kManyThreads, 1)
 expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams p) {
     constexpr uint32_t SPB = (BITS == 8 ? 128 : 256) / KS;   // steps per raw block
     constexpr uint32_t kSlotCols = KS / 2;                   // TMEM columns of a step's weights
     constexpr uint32_t kSlots = slots(KS, LOW);
-    constexpr Shares kShares = shares(CG, BITS == 4 && GROUPED);
-    constexpr int kConvGroups = CG, kFirstLoad = kFirstConv + 4 * CG;
+    constexpr Shares kShares = shares(BITS == 4 && GROUPED);
     constexpr uint32_t kIssuers = LOW ? 2 : 1;
-    static_assert(!LOW || (CG == 4 && kSlots % 2 == 0), "a slot's steps are one issuer's");
+    static_assert(!LOW || (kConvGroups % 2 == 0 && kSlots % 2 == 0), "a slot's steps are one issuer's");
     extern __shared__ uint8_t smem_raw_base[];
     const uint32_t smem_base = (ptx::smem_u32(smem_raw_base) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw_base + (smem_base - ptx::smem_u32(smem_raw_base));
@@ -223,7 +223,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
     if (warp == 0 && lane == 0) {
         for (uint32_t s = 0; s < p.raw_stages; ++s) { ptx::mbar_init(raw_full(s), 1); ptx::mbar_init(raw_empty(s), 4 * SPB); }
         for (uint32_t s = 0; s < kSlots; ++s) { ptx::mbar_init(step_full(s), 4 + 32 * kLoadWarps + (rank == 0 ? 1 : 0)); ptx::mbar_init(step_empty(s), 1); }
-        for (uint32_t s = 0; s < (LOW ? 2u : p.accs); ++s) { ptx::mbar_init(acc_full(s), 1); ptx::mbar_init(acc_empty(s), 2 * kEpiWarps); }
+        for (uint32_t s = 0; s < kIssuers; ++s) { ptx::mbar_init(acc_full(s), 1); ptx::mbar_init(acc_empty(s), 2 * kEpiWarps); }
         *abort_flag = 0;
         ptx::fence_mbar_init();
         ptx::prefetch_tmap(&tmap_w);
@@ -311,7 +311,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                     }
                 }
                 before += ns;
-                rc.step(1, p.accs);
+                rc.step(1, 1);
             }
         } else if (warp == 2) {
             // ======================= rank 1: reports its half of each step =======================
@@ -582,7 +582,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                 finish(o[i], v, 16 * i);
             }
             drained();
-            rc.step(1, p.accs);
+            rc.step(1, 1);
             // Blocks of 16 rows turn round in shared memory and leave in 16-byte pieces, 64 (gated 32) contiguous bytes a row; two blocks take turns.
             const uint32_t c0 = x.n0 + quarter * 32u;   // first channel of this warp
             if (c0 >= p.x.n) continue;
@@ -645,21 +645,21 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
     }
 }
 
-template <int BITS, bool GROUPED, int KS, int CG, bool LOW>
-int launch_groups(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uint32_t smem, DeviceCtx* ctx, cudaStream_t s) {
-    auto kern = expert_many_kernel<BITS, GROUPED, KS, CG, LOW>;
+template <int BITS, bool GROUPED, int KS, bool LOW>
+int launch_many(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uint32_t smem, DeviceCtx* ctx, cudaStream_t s) {
+    auto kern = expert_many_kernel<BITS, GROUPED, KS, LOW>;
     static DeviceOnce attr_set;  // per template instance
     if (!attr_set.done(ctx->device)) {
         cudaFuncAttributes attr;
         cudaError_t e = cudaFuncGetAttributes(&attr, kern);
         if (e != cudaSuccess) return cuda_fail(e);
-        if ((uint32_t)(attr.numRegs * many_threads(CG)) < regs_all(CG, BITS == 4 && GROUPED)) return AFB_ERR_UNSUPPORTED;   // the shares come out of what the block is launched with
+        if ((uint32_t)(attr.numRegs * kManyThreads) < regs_all(BITS == 4 && GROUPED)) return AFB_ERR_UNSUPPORTED;   // the shares come out of what the block is launched with
         e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
         if (e != cudaSuccess) return cuda_fail(e);
         attr_set.mark(ctx->device);
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(many_threads(CG)); cfg.stream = s; cfg.dynamicSmemBytes = smem;
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(kManyThreads); cfg.stream = s; cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
@@ -673,8 +673,7 @@ int launch_groups(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uin
 
 template <int BITS, bool GROUPED, int KS>
 int launch_cfg(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uint32_t smem, DeviceCtx* ctx, cudaStream_t s) {
-    if (p.x.tile_rows <= 64) return launch_groups<BITS, GROUPED, KS, 4, true>(tw, p, grid, smem, ctx, s);
-    return p.x.tile_rows <= 128 ? launch_groups<BITS, GROUPED, KS, 4, false>(tw, p, grid, smem, ctx, s) : launch_groups<BITS, GROUPED, KS, 2, false>(tw, p, grid, smem, ctx, s);
+    return p.x.tile_rows <= 64 ? launch_many<BITS, GROUPED, KS, true>(tw, p, grid, smem, ctx, s) : launch_many<BITS, GROUPED, KS, false>(tw, p, grid, smem, ctx, s);
 }
 
 }  // namespace
@@ -687,13 +686,13 @@ int launch_expert_many(const ExpertParams& q, uint32_t bits, uint32_t group, Dev
     p.x.set_blocks((q.n + 2 * kCh - 1) / (2 * kCh));
     p.steps = q.k / ks;
     const uint32_t per_block = p.steps % spb == 0 ? spb : 1;
-    // Up to 128 rows there are two accumulators, and twice the raw blocks under way.  Up to 64 each of two issuers has one, in return for six slots (four, and two
-    // accumulators each: 843 cycles per step, of which the converters' turn, 2200 from a free slot to the next, is the most); whole raw blocks
-    // only (see below), and a step for each issuer.
-    p.x.tile_rows = (uint64_t)q.m <= 40ull * q.experts && per_block == spb && p.steps > 1 ? 64 : (uint64_t)q.m <= 160ull * q.experts ? 128 : 256;
+    // Strips of up to 64 rows leave room for six slots and an accumulator for each of two issuers (whole raw blocks only, see below, and a step for each issuer).
+    // By the mean of the rows per expert (us, strips up to 64 / up to 256): 64 experts of 2048 x 4096, int4 group-128: 16 rows 114 / 122, 32: 130 / 136, 40: 144 / 140;
+    // int8: 16: 103 / 111, 40: 119 / 127, 48: 125 / 123;  39 of 8368 x 2176, int8: 32: 146 / 150, 40: 160 / 156.  (Strips up to 128 with two accumulators of one
+    // issuer take more steps: 48 rows, int4: 142; 140: 222 where strips up to 256 take 206.)
+    p.x.tile_rows = (uint64_t)q.m <= 36ull * q.experts && per_block == spb && p.steps > 1 ? 64 : 256;
     const bool low = p.x.tile_rows <= 64;
     const uint32_t kSlots = slots(ks, low);
-    p.accs = p.x.tile_rows <= 64 || p.x.tile_rows > 128 ? 1 : 2;
     p.off_raw = (kOffTable + ExpertTable::bytes(q.experts) + 1023u) / 1024u * 1024u;
     const uint32_t act_bytes = kSlots * p.x.tile_rows * ks;
     p.raw_stages = (232448 - 1024 - p.off_raw - act_bytes) / kRawBytes;
@@ -701,7 +700,6 @@ int launch_expert_many(const ExpertParams& q, uint32_t bits, uint32_t group, Dev
     // The parity waits of the converters: see stream.cu.  With two issuers a free slot tells about every second step only; so of the raw blocks either
     // every one has a step of each issuer, or the ring is of an even number of blocks with a step each, and the block that had its place in the
     // ring before had one of the same issuer's.
-    const uint32_t kConvGroups = p.x.tile_rows <= 128 ? 4 : 2;
     if (low && spb == 1) p.raw_stages &= ~1u;
     p.slot_first = !low && p.raw_stages * per_block >= kConvGroups + kSlots + per_block - 1 ? 0u : 1u;
     if (p.raw_stages * per_block < kSlots + per_block - 1) return AFB_ERR_UNSUPPORTED;   // not with any size that this function takes
