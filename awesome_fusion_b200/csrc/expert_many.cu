@@ -287,13 +287,13 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
             const uint32_t who = (uint32_t)warp - 2;
             const uint64_t desc0 = ptx::umma_desc_kmajor_sw128(smem_base + off_act);
             r.i = who;
-            Ring rc{0, 0};
+            Ring rc{0, 0};   // the accumulator(s): a ring of one
             uint32_t before = 0, g = who;   // steps of the tiles walked so far; this warp's next step, counted over all tiles
             bool ready = false;
             while (ok && next(x)) {
                 const uint32_t idesc = GROUPED ? ptx::umma_idesc_f16_f32(2 * kCh, x.height) : ptx::umma_idesc_bf16_f32(2 * kCh, x.height), slab_d = x.height * 64u >> 4;
-                const uint32_t acc = LOW ? who : rc.i, td = tmem_base + acc * acc_cols, acc_done = acc_full(acc), first = g;
-                if (!warp_wait(acc_empty(acc), rc.phase ^ 1u, abort_flag)) { give_up(63, x.expert, 0); break; }
+                const uint32_t td = tmem_base + who * acc_cols, acc_done = acc_full(who), first = g;
+                if (!warp_wait(acc_empty(who), rc.phase ^ 1u, abort_flag)) { give_up(63, x.expert, 0); break; }
                 for (; g < before + ns; g += kIssuers) {
                     if (!__all_sync(0xffffffffu, ready) && !warp_wait(step_full(r.i), r.phase, abort_flag)) { give_up(64, x.expert, g); ok = false; break; }
                     ptx::fence_proxy_async_smem();
@@ -497,7 +497,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
         constexpr int kPacks = LOW ? 2 : 8;   // of 16 columns: this warp's half of a strip
         const bool odd = lane & 1, gated = p.x.gated != 0, act = p.x.silu != 0;
         const uint32_t stage = smem_base + kOffOut + (uint32_t)(warp - kFirstEpi) * 2 * kOutBytes;
-        Ring rc{0, 0};
+        Ring rc{0, 0};   // the accumulator(s): a ring of one
         bool ok = true;
         auto drained = [&] {   // everything of the accumulator is in registers
             ptx::tc_fence_before_sync();
@@ -505,7 +505,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
             if (lane == 0) {
 #pragma unroll
                 for (uint32_t h = 0; h < kIssuers; ++h) {
-                    const uint32_t b = acc_empty(LOW ? h : rc.i);
+                    const uint32_t b = acc_empty(h);
                     if (rank == 0) ptx::mbar_arrive(b); else ptx::mbar_arrive_remote(b, 0);
                 }
             }
@@ -557,7 +557,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                 const uint32_t row = i * 32 + lane < valid ? p.x.row_pair ? source_row(p.x, x.row0 + first + i * 32 + lane) : x.row0 + first + i * 32 + lane : 0xffffffffu;
                 factor[i] = GROUPED && row < p.x.a_rows ? p.row_factor[row] * 512.f : 0.f;
             }
-            if (!warp_wait(acc_full(rc.i), rc.phase, abort_flag)) { give_up(68, x.expert, 0); break; }
+            if (!warp_wait(acc_full(0), rc.phase, abort_flag)) { give_up(68, x.expert, 0); break; }
             if (LOW && !warp_wait(acc_full(1), rc.phase, abort_flag)) { give_up(68, x.expert, 1); break; }
             ptx::tc_fence_after_sync();
 #pragma unroll
@@ -573,7 +573,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
 #pragma unroll
                     for (int j = 0; j < 16; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) + __uint_as_float(b[j]));
                 } else {
-                    ptx::tmem_ld_32x16(column + rc.i * acc_cols + 16 * i, a);
+                    ptx::tmem_ld_32x16(column + 16 * i, a);
                     ptx::tmem_ld_wait();
                 }
 #pragma unroll

@@ -455,6 +455,20 @@ def test_expert_gemm_of_many_experts(afb, variant, bits, group):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("variant", FORMS)
+@pytest.mark.parametrize("fmt", [dict(bits=8), dict(bits=8, group=64), dict(bits=4, group=128, packed=True)], ids=lambda f: "-".join(f"{k}{v}" for k, v in f.items()))
+def test_expert_gemm_after_a_call_full_of_nan(afb, variant, fmt):
+    """Where a strip has places for more rows than the expert has, shared memory holds what an earlier launch left there: rows of NaN here."""
+    x = Experts(8, 2304, 1024, seed=23, **fmt)
+    full, counts = [32] * 8, [1, 5, 17, 0, 31, 2, 3, 9]
+    offsets, a = offsets_of(counts), activations(sum(counts), 1024)
+    want = x.plain(a, offsets, variant=variant)
+    assert x.run(afb, torch.full((sum(full), 1024), math.nan, device="cuda", dtype=torch.bfloat16), offsets_of(full), variant=variant).isnan().all()
+    check(x.run(afb, a, offsets, variant=variant), *want)
+    assert afb.read_status()[0] == 0
+
+
+@pytest.mark.gpu
 def test_expert_gemm_without_workspace(afb):
     """cudaStreamPerThread names no stream to keep a workspace for: the form for few rows takes what would need one."""
     x = Experts(2, 72, 256, 4, 128, seed=19)
