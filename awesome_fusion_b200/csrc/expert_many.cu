@@ -25,7 +25,7 @@
 //
 // What bounds it.  Strips of 256 rows: the tensor pipe, under the power limit (8192 rows on 8 experts of 22016 x 4096 int8, gated: 1047 us = 1.41 PFLOP/s), and per tile
 // the drain of the only accumulator (2000 to 3000 cycles); where they are lower than that the hand-offs (16384 rows on 64 experts of 2048 x 4096 int4 group-128: 274 us
-// = 1.0 PFLOP/s).  Strips up to 64: int4 in groups by instructions, 0.69 of the issue slots (1024 rows: 114 us; a group of converters needs 2600 cycles for a
+// = 1.0 PFLOP/s).  Strips up to 64: int4 in groups by instructions, 0.66 of the issue slots (1024 rows: 114 us; a group of converters needs 2600 cycles for a
 // step, four of them at a time); int8 per channel by HBM (103 us, 5.2 TB/s of weights).
 #include <cuda_fp16.h>
 #include "dequant.cuh"
