@@ -355,6 +355,7 @@ using namespace afb;
 
 extern "C" int afb_moe_route_workspace(uint32_t tokens, uint32_t experts, uint64_t* bytes) {
     if (!bytes || experts == 0 || experts > AFB_MOE_MAX_EXPERTS) return AFB_ERR_BAD_ARG;
+    if (tokens >> 31) return AFB_ERR_TOO_LARGE;   // no route has as many; the block sizes below would leave 32 bits
     // also for sizes that one CTA takes: top_k decides, and it is not asked for here
     const uint64_t blocks = tokens ? (tokens + route_block_tokens(tokens) - 1) / route_block_tokens(tokens) : 0;
     *bytes = one_block(tokens, experts < AFB_MOE_MAX_TOP_K ? experts : AFB_MOE_MAX_TOP_K) ? 0 : blocks * experts * sizeof(int32_t);

@@ -237,7 +237,8 @@ typedef struct afb_moe_route_args {
     uint32_t  renormalize;     /* 0 / 1                                                                             */
     uint64_t  reserved;        /* must be 0                                                                         */
 } afb_moe_route_args;
-/* Bytes of device memory that a route of this size needs at ptr_workspace (0: none; then NULL will do).  Needs no GPU. */
+/* Bytes of device memory that a route of this size needs at ptr_workspace (0: none; then NULL will do).  Needs no GPU.
+ * AFB_ERR_TOO_LARGE from 2^31 tokens on. */
 int afb_moe_route_workspace(uint32_t tokens, uint32_t experts, uint64_t* bytes);
 int afb_moe_route_launch(const afb_moe_route_args* args, void* stream);
 /* afb_expert_gemm_launch.  gemm describes one expert's product, with
