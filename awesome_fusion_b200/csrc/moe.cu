@@ -401,7 +401,7 @@ extern "C" int afb_moe_route_launch(const afb_moe_route_args* a, void* stream) {
 
 extern "C" int afb_moe_combine_launch(const afb_moe_combine_args* a, void* stream) {
     if (!a || a->reserved != 0 || a->top_k == 0 || a->n == 0) return AFB_ERR_BAD_ARG;
-    if (a->n >> 31) return AFB_ERR_TOO_LARGE;
+    if (a->n >> 31 || a->tokens >> 31) return AFB_ERR_TOO_LARGE;   // the blocks' stride over the tokens stays in 32 bits
     if (a->tokens == 0) return AFB_OK;
     if (!a->ptr_out || !a->ptr_weights || !a->ptr_pair_row || (a->rows && !a->ptr_y)) return AFB_ERR_BAD_ARG;
     if ((uintptr_t)a->ptr_out % 2 || (uintptr_t)a->ptr_y % 2 || (uintptr_t)a->ptr_residual % 2 || (uintptr_t)a->ptr_weights % 4 || (uintptr_t)a->ptr_pair_row % 4) return AFB_ERR_BAD_ARG;

@@ -280,7 +280,7 @@ typedef struct afb_moe_combine_args {
     const float*   ptr_weights;    /* [tokens, top_k] */
     const int32_t* ptr_pair_row;   /* [tokens, top_k] */
     const void*    ptr_residual;   /* bf16 [tokens, n], ld_residual; or NULL */
-    uint32_t tokens, top_k, rows, n;
+    uint32_t tokens, top_k, rows, n;   /* tokens, n < 2^31 */
     uint32_t ld_out, ld_y, ld_residual;
     uint32_t reserved;             /* must be 0 */
 } afb_moe_combine_args;
