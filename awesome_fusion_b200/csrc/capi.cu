@@ -43,7 +43,15 @@ void count_pair_launch() { g_pair_launches.fetch_add(1); }
 DeviceCtx* current_ctx() {
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return nullptr;
-    return g_ctx[dev].ready ? &g_ctx[dev] : nullptr;
+    if (!g_ctx[dev].ready) return nullptr;
+    // A thread that has not used the device yet has no current context, and encoding a tensor map, often a call's first step, asks for one
+    // without making it.
+    static thread_local int current = -1;
+    if (current != dev) {
+        if (cudaSetDevice(dev) != cudaSuccess) { (void)cudaGetLastError(); return nullptr; }
+        current = dev;
+    }
+    return &g_ctx[dev];
 }
 
 unsigned long long* phase_ts_if_enabled(DeviceCtx* ctx) {
