@@ -47,6 +47,7 @@ struct DeviceCtx {
     int          kept_graph_workspaces = 0;     // taken by graphs for good
     size_t       stream_counter_count = 0;      // counters of every one
     cudaStream_t clear_stream = nullptr;        // clears the counters of a workspace that is taken inside a capture
+    cudaMemPool_t call_pool = nullptr;          // what CallMemory hands out
     // optional phase timestamps (globaltimer ns of THIS GPU) written by the row-parallel GEMM and the exchange kernel when the
     // environment variable AFB_PHASE_TIMESTAMPS is set: [0] GEMM start, [1] GEMM end (latest CTA), [2] exchange start,
     // [3] all ranks' GEMMs seen complete, [4] sum + broadcast done (latest CTA), [5] all ranks' blocks seen in place
@@ -77,10 +78,26 @@ DeviceCtx* current_ctx();           // nullptr when afb_init was not called on t
 const DeviceCtx::Workspace* workspace_for(DeviceCtx* ctx, cudaStream_t s, int* rc);
 // A workspace of at least `bytes` for a streaming launch on `s`; false: there is none to be had, the caller takes another form.
 bool stream_workspace(DeviceCtx* ctx, cudaStream_t s, size_t bytes, float** ws, uint32_t** counters);
+// Memory that one call's launches on `s` hand results through, no other call's while it lives: several launches are not one, and another
+// thread's may come between them on the same stream.  Taken and given back in the order of the stream; inside a capture it is the graph's
+// workspace, which no launch outside the graph sees.  get() is nullptr where there is none to be had.
+class CallMemory {
+public:
+    CallMemory(DeviceCtx* ctx, cudaStream_t s, size_t bytes);
+    ~CallMemory();
+    CallMemory(const CallMemory&) = delete;
+    CallMemory& operator=(const CallMemory&) = delete;
+    void* get() const { return ptr_; }
+private:
+    void*        ptr_ = nullptr;
+    cudaStream_t stream_;
+    bool         pooled_ = false;
+};
 int  cuda_fail(cudaError_t e);      // records e, returns AFB_ERR_CUDA
 void count_launch(unsigned n = 1);
 void count_stream_launch();          // of the streaming form (counted by count_launch as well)
 void count_pair_launch();            // of the pair form (likewise)
+void count_expert_many_launch();     // of the products grouped by expert, form for many rows (likewise)
 
 // Driver entry point for tensor-map encoding, fetched once through the runtime.
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,

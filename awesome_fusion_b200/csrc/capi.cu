@@ -15,7 +15,7 @@ constexpr int kMaxDevices = 32;
 DeviceCtx g_ctx[kMaxDevices];
 std::mutex g_mutex;
 std::atomic<int> g_last_cuda_error{0};
-std::atomic<unsigned long long> g_launches{0}, g_stream_launches{0}, g_pair_launches{0};
+std::atomic<unsigned long long> g_launches{0}, g_stream_launches{0}, g_pair_launches{0}, g_expert_many_launches{0};
 constexpr size_t kSplitKWorkspaceBytes = 32u << 20;
 constexpr size_t kSplitKCounters = 4096;
 constexpr int kPreallocatedWorkspaces = 8;
@@ -28,6 +28,8 @@ constexpr int kKeptGraphWorkspaces = 32;
 // Of a stream: two partial sums per SM of a tile of 256 rows (the pair form's highest, the streaming form's is 192) x 128 channels.  A stream
 // takes it once and for both forms, so that its later launches allocate nothing.
 size_t stream_workspace_bytes(int sm_count) { return (size_t)2 * sm_count * 256 * 128 * sizeof(float); }
+// What CallMemory's pool keeps when the device has been waited for and nothing is in use; a call that needs more has it mapped anew after each wait.
+constexpr uint64_t kCallMemoryKept = 1024u << 20;
 constexpr uint32_t kPrefillTsMinM = 128;   // measured: above 128 activation rows the tensor-memory form is 1.3x faster, at 128 it is slower
 }  // namespace
 
@@ -39,6 +41,7 @@ int cuda_fail(cudaError_t e) {
 void count_launch(unsigned n) { g_launches.fetch_add(n); }
 void count_stream_launch() { g_stream_launches.fetch_add(1); }
 void count_pair_launch() { g_pair_launches.fetch_add(1); }
+void count_expert_many_launch() { g_expert_many_launches.fetch_add(1); }
 
 DeviceCtx* current_ctx() {
     int dev = -1;
@@ -187,6 +190,34 @@ bool stream_workspace(DeviceCtx* ctx, cudaStream_t s, size_t bytes, float** ws, 
     return true;
 }
 
+CallMemory::CallMemory(DeviceCtx* ctx, cudaStream_t s, size_t bytes) : stream_(s) {
+    if (s == cudaStreamPerThread) return;   // as of stream_workspace
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(s, &status) != cudaSuccess) { (void)cudaGetLastError(); return; }
+    if (status != cudaStreamCaptureStatusNone) {
+        float* ws = nullptr;
+        uint32_t* counters;
+        if (stream_workspace(ctx, s, bytes, &ws, &counters)) ptr_ = ws;
+        return;
+    }
+    if (!ctx->call_pool) return;
+    RelaxedCapture relaxed;
+    cudaError_t e = cudaMallocFromPoolAsync(&ptr_, bytes, ctx->call_pool, s);
+    if (e == cudaErrorMemoryAllocation) {   // what the pool keeps in other sizes may be what is missing
+        (void)cudaGetLastError();
+        (void)cudaMemPoolTrimTo(ctx->call_pool, 0);
+        e = cudaMallocFromPoolAsync(&ptr_, bytes, ctx->call_pool, s);
+    }
+    if (e != cudaSuccess) { (void)cuda_fail(e); ptr_ = nullptr; return; }
+    pooled_ = true;
+}
+CallMemory::~CallMemory() {
+    if (!pooled_) return;
+    RelaxedCapture relaxed;
+    const cudaError_t e = cudaFreeAsync(ptr_, stream_);
+    if (e != cudaSuccess) (void)cuda_fail(e);
+}
+
 const DeviceCtx::Workspace* workspace_for(DeviceCtx* ctx, cudaStream_t s, int* rc) {
     std::lock_guard<std::mutex> lock(g_mutex);
     DeviceCtx::Workspace* free_slot = nullptr;
@@ -295,6 +326,19 @@ int afb_init(int device) {
     c.stream_counter_count = 3 * (size_t)c.sm_count;   // a launch shares fewer than two tiles per SM, of pairs of SMs fewer than one and three words a rank
     AFB_CUDA(allocate_stream_workspace(&c, &c.stream_workspaces[0], stream_workspace_bytes(c.sm_count)));   // the first stream's
     AFB_CUDA(cudaStreamCreateWithFlags(&c.clear_stream, cudaStreamNonBlocking));
+    int pools = 0;
+    AFB_CUDA(cudaDeviceGetAttribute(&pools, cudaDevAttrMemoryPoolsSupported, device));
+    if (pools) {
+        cudaMemPoolProps props = {};
+        props.allocType = cudaMemAllocationTypePinned;
+        props.location.type = cudaMemLocationTypeDevice;
+        props.location.id = device;
+        AFB_CUDA(cudaMemPoolCreate(&c.call_pool, &props));
+        uint64_t kept = kCallMemoryKept;
+        int wait = 0;   // a stream never waits for another one's memory
+        AFB_CUDA(cudaMemPoolSetAttribute(c.call_pool, cudaMemPoolAttrReleaseThreshold, &kept));
+        AFB_CUDA(cudaMemPoolSetAttribute(c.call_pool, cudaMemPoolReuseAllowInternalDependencies, &wait));
+    }
     AFB_CUDA(cudaMalloc(&c.phase_ts, 8 * sizeof(unsigned long long)));
     AFB_CUDA(cudaMemset(c.phase_ts, 0, 8 * sizeof(unsigned long long)));
     AFB_CUDA(cudaMalloc(&c.ar_words, 4 * sizeof(uint32_t)));
@@ -315,6 +359,7 @@ int afb_finalize(void) {
     for (auto& w : c.workspaces) { if (w.ws) cudaFree(w.ws); if (w.counters) cudaFree(w.counters); }
     for (auto& w : c.stream_workspaces) { if (w.counters) cudaFree(w.counters); if (w.hold) w.hold->release(); }
     if (c.clear_stream) cudaStreamDestroy(c.clear_stream);
+    if (c.call_pool) cudaMemPoolDestroy(c.call_pool);
     for (int j = 0; j < 2; ++j) {
         for (int i = 0; i < 4; ++i) if (c.stage[j][i]) cudaFree(c.stage[j][i]);
         if (c.stage_free[j]) cudaEventDestroy(c.stage_free[j]);
@@ -651,6 +696,7 @@ const char* afb_last_cuda_error_string(void) { return cudaGetErrorString((cudaEr
 unsigned long long afb_launch_count(void) { return g_launches.load(); }
 unsigned long long afb_stream_launch_count(void) { return g_stream_launches.load(); }
 unsigned long long afb_pair_launch_count(void) { return g_pair_launches.load(); }
+unsigned long long afb_expert_many_launch_count(void) { return g_expert_many_launches.load(); }
 const char* afb_version(void) { return "afb 0.1 (sm_100a)"; }
 
 }  // extern "C"

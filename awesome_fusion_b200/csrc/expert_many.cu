@@ -668,6 +668,7 @@ int launch_many(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uint3
     cfg.attrs = attr; cfg.numAttrs = GROUPED ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, p);
     count_launch();
+    count_expert_many_launch();
     return e == cudaSuccess ? AFB_OK : cuda_fail(e);
 }
 
@@ -709,35 +710,36 @@ int launch_expert_many(const ExpertParams& q, uint32_t bits, uint32_t group, Dev
     if (tiles >> 31) { *done = true; return AFB_ERR_TOO_LARGE; }
     const uint32_t pairs = (uint32_t)ctx->sm_count / 2, grid = 2 * (tiles < pairs ? (uint32_t)tiles : pairs);
     const uint32_t smem = 1024 + p.off_raw + p.raw_stages * kRawBytes + act_bytes;
-    if (group) {
-        // rows of A, their factors, the channels' multipliers, each from a multiple of 256 bytes on
-        const uint64_t a_bytes = ((uint64_t)q.a_rows * q.k * 2 + 255) / 256 * 256, row_bytes = ((uint64_t)q.a_rows * 4 + 255) / 256 * 256;
-        const uint64_t channels = (uint64_t)q.experts * q.n;
-        float* ws;
-        uint32_t* counters;
-        if (!stream_workspace(ctx, s, a_bytes + row_bytes + channels * 4, &ws, &counters)) return AFB_OK;
-        PrepareParams prep{};
-        prep.x = q;
-        prep.a = reinterpret_cast<uint16_t*>(ws);
-        prep.row_factor = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + a_bytes);
-        prep.channel_mult = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + a_bytes + row_bytes);
-        prep.channel_blocks = (uint32_t)((channels + kPrepareThreads - 1) / kPrepareThreads);
-        for (prep.row_threads = 32; prep.row_threads < (uint32_t)kPrepareThreads && prep.row_threads * kHeld * 8 < q.k;) prep.row_threads *= 2;
-        const uint32_t rows = kPrepareThreads / prep.row_threads;
-        expert_prepare_kernel<<<prep.channel_blocks + (q.a_rows + rows - 1) / rows, kPrepareThreads, 0, s>>>(prep);
-        count_launch();
-        const cudaError_t e = cudaGetLastError();
-        if (e != cudaSuccess) { *done = true; return cuda_fail(e); }
-        p.x.a = prep.a; p.x.lda = q.k;
-        p.row_factor = prep.row_factor; p.channel_mult = prep.channel_mult;
-    }
-    *done = true;
     CUtensorMap tw;
     const int rc = tmap_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.b, (uint64_t)q.k * bits / 8, (uint64_t)q.experts * q.n, q.ldb_bytes, 128, kCh, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc) return rc;
-    if (bits == 4) return group ? launch_cfg<4, true, 128>(tw, p, grid, smem, ctx, s) : launch_cfg<4, false, 128>(tw, p, grid, smem, ctx, s);   // k is a multiple of 128
-    if (group) return ks == 128 ? launch_cfg<8, true, 128>(tw, p, grid, smem, ctx, s) : launch_cfg<8, true, 64>(tw, p, grid, smem, ctx, s);
-    return ks == 128 ? launch_cfg<8, false, 128>(tw, p, grid, smem, ctx, s) : launch_cfg<8, false, 64>(tw, p, grid, smem, ctx, s);
+    if (rc) { *done = true; return rc; }
+    if (!group) {
+        *done = true;
+        if (bits == 4) return launch_cfg<4, false, 128>(tw, p, grid, smem, ctx, s);   // k is a multiple of 128
+        return ks == 128 ? launch_cfg<8, false, 128>(tw, p, grid, smem, ctx, s) : launch_cfg<8, false, 64>(tw, p, grid, smem, ctx, s);
+    }
+    // rows of A, their factors, the channels' multipliers, each from a multiple of 256 bytes on
+    const uint64_t a_bytes = ((uint64_t)q.a_rows * q.k * 2 + 255) / 256 * 256, row_bytes = ((uint64_t)q.a_rows * 4 + 255) / 256 * 256;
+    const uint64_t channels = (uint64_t)q.experts * q.n;
+    const CallMemory memory(ctx, s, a_bytes + row_bytes + channels * 4);   // given back behind the second launch
+    if (!memory.get()) return AFB_OK;
+    *done = true;
+    PrepareParams prep{};
+    prep.x = q;
+    prep.a = reinterpret_cast<uint16_t*>(memory.get());
+    prep.row_factor = reinterpret_cast<float*>(reinterpret_cast<char*>(memory.get()) + a_bytes);
+    prep.channel_mult = reinterpret_cast<float*>(reinterpret_cast<char*>(memory.get()) + a_bytes + row_bytes);
+    prep.channel_blocks = (uint32_t)((channels + kPrepareThreads - 1) / kPrepareThreads);
+    for (prep.row_threads = 32; prep.row_threads < (uint32_t)kPrepareThreads && prep.row_threads * kHeld * 8 < q.k;) prep.row_threads *= 2;
+    const uint32_t rows = kPrepareThreads / prep.row_threads;
+    expert_prepare_kernel<<<prep.channel_blocks + (q.a_rows + rows - 1) / rows, kPrepareThreads, 0, s>>>(prep);
+    count_launch();
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e);
+    p.x.a = prep.a; p.x.lda = q.k;
+    p.row_factor = prep.row_factor; p.channel_mult = prep.channel_mult;
+    if (bits == 4) return launch_cfg<4, true, 128>(tw, p, grid, smem, ctx, s);
+    return ks == 128 ? launch_cfg<8, true, 128>(tw, p, grid, smem, ctx, s) : launch_cfg<8, true, 64>(tw, p, grid, smem, ctx, s);
 }
 
 }  // namespace afb

@@ -209,8 +209,8 @@ int afb_prepack_gated(const afb_gemm_args* gate, const void* b_up, const void* s
  *     afb_moe_route_launch    logits -> picks, weights, and the pairs (token, pick) sorted by expert
  *     afb_expert_gemm_launch  the products grouped by expert, once for gate and up projection (gated), once for the down projection
  *     afb_moe_combine_launch  the weighted sum of the picked experts' answers
- * All four launches of a layer go to one stream; nothing is copied to the host, no size depends on the picks, nothing is allocated, so
- * the layer can be captured in a graph.  A pair is numbered token * top_k + pick; the ROW of a pair is its place in the sorted order.
+ * All four go to one stream; nothing is copied to the host and no size depends on the picks, so the layer can be captured in a graph.
+ * Nothing is allocated but what afb_expert_gemm_launch says.  Any number of host threads may call, also on one stream.  A pair is numbered token * top_k + pick; the ROW of a pair is its place in the sorted order.
  *
  * afb_moe_route_launch.  For every token the top_k largest logits in falling order, of equal ones the lower expert first (-0 equals 0).
  * A logit that is -inf or NaN is masked: its expert is never picked.  Where fewer than top_k experts are left (none in a token of padding)
@@ -256,8 +256,10 @@ int afb_moe_route_launch(const afb_moe_route_args* args, void* stream);
  * in fp32 from the fp32 sums, rounded to bf16 once.  Group scales multiply the fp32 sum of each group in the form for few rows.  In the form for many they
  * multiply the weights, in fp16: the product is exact for int4 without zero-points and bf16 scales, else off by 2^-11 of itself at most (2^-10 for fp32
  * scales); rows of A and the scales of a channel are given a power of two for that, and of the row's values what is below 2^-28 of the largest (of the
- * scales 2^-20) keeps fewer bits.  This form converts the rows of A into a workspace of the stream or captured graph first, as the streaming form
- * has one; where there is none to be had the other form runs.
+ * scales 2^-20) keeps fewer bits.  This form converts the rows of A first, into a_rows * k * 2 bytes and a little that the call takes and gives back in
+ * the order of the stream (cudaMallocFromPoolAsync; the library's pool keeps up to 1 GB of what was used); inside a capture into a workspace of
+ * the graph, as the streaming form has one.  Where there is no such memory to be had, and on cudaStreamPerThread, the other form runs
+ * (afb_expert_many_launch_count tells).
  * The offsets are read on the GPU.  They must not fall; values outside 0 .. m are taken as the nearer end.  A row(r) outside
  * 0 .. a_rows - 1 reads as a row of zeros. */
 typedef struct afb_expert_gemm_args {
@@ -432,6 +434,8 @@ unsigned long long afb_launch_count(void);
 unsigned long long afb_stream_launch_count(void);
 /* ... and of the pair form of the prefill variant and the fused launches */
 unsigned long long afb_pair_launch_count(void);
+/* ... and of the products grouped by expert in the form for many rows */
+unsigned long long afb_expert_many_launch_count(void);
 const char* afb_version(void);
 
 #ifdef __cplusplus
