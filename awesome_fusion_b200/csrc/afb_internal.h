@@ -48,6 +48,15 @@ struct DeviceCtx {
     size_t       stream_counter_count = 0;      // counters of every one
     cudaStream_t clear_stream = nullptr;        // clears the counters of a workspace that is taken inside a capture
     cudaMemPool_t call_pool = nullptr;          // what CallMemory hands out
+    struct GraphMemory {                        // ... to the calls of a capture
+        void*              ptr;
+        size_t             bytes;
+        cudaStream_t       stream;
+        unsigned long long capture;
+        GraphHold*         hold;
+        GraphMemory*       next;
+    };
+    GraphMemory* graph_memory = nullptr;
     // optional phase timestamps (globaltimer ns of THIS GPU) written by the row-parallel GEMM and the exchange kernel when the
     // environment variable AFB_PHASE_TIMESTAMPS is set: [0] GEMM start, [1] GEMM end (latest CTA), [2] exchange start,
     // [3] all ranks' GEMMs seen complete, [4] sum + broadcast done (latest CTA), [5] all ranks' blocks seen in place
@@ -79,8 +88,8 @@ const DeviceCtx::Workspace* workspace_for(DeviceCtx* ctx, cudaStream_t s, int* r
 // A workspace of at least `bytes` for a streaming launch on `s`; false: there is none to be had, the caller takes another form.
 bool stream_workspace(DeviceCtx* ctx, cudaStream_t s, size_t bytes, float** ws, uint32_t** counters);
 // Memory that one call's launches on `s` hand results through, no other call's while it lives: several launches are not one, and another
-// thread's may come between them on the same stream.  Taken and given back in the order of the stream; inside a capture it is the graph's
-// workspace, which no launch outside the graph sees.  get() is nullptr where there is none to be had.
+// thread's may come between them on the same stream.  Taken and given back in the order of the stream; inside a capture it is the graph's,
+// for as long as there is the graph or an executable of it.  get() is nullptr where there is none to be had.
 class CallMemory {
 public:
     CallMemory(DeviceCtx* ctx, cudaStream_t s, size_t bytes);

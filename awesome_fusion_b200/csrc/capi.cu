@@ -20,7 +20,6 @@ constexpr size_t kSplitKWorkspaceBytes = 32u << 20;
 constexpr size_t kSplitKCounters = 4096;
 constexpr int kPreallocatedWorkspaces = 8;
 constexpr size_t kMinStreamWorkspace = 4u << 20;       // of a captured graph: a power of two from here on
-constexpr size_t kMaxStreamWorkspace = 1024u << 20;
 constexpr size_t kMaxStreamWorkspaceTotal = 3072u << 20;   // 79 streams of 148 SMs; beyond this, and beyond kMaxStreamWorkspaces, launches take another form
 // Captured graphs whose workspaces stay theirs until afb_finalize, as streams' do.  Those of further graphs go back to the pool when the
 // graph is gone; the user object that says so costs each replay of the graph 2.5 us (16 x 22016 x 4096 int4, captured: 30.9 / 33.9 us).
@@ -136,10 +135,9 @@ bool stream_workspace(DeviceCtx* ctx, cudaStream_t s, size_t bytes, float** ws, 
     std::lock_guard<std::mutex> lock(g_mutex);
     // a stream's own workspace serves all its launches to come, a graph's the one at hand and those no larger
     const size_t whole = stream_workspace_bytes(ctx->sm_count);
-    if (bytes > kMaxStreamWorkspace) return false;
+    if (bytes > whole) return false;
     size_t want = whole;
-    if (bytes > whole) while (want < bytes) want *= 2;   // the converted activations of products grouped by expert
-    else if (capturing) for (want = kMinStreamWorkspace; want < bytes;) want = want * 2 < whole ? want * 2 : whole;
+    if (capturing) for (want = kMinStreamWorkspace; want < bytes;) want = want * 2 < whole ? want * 2 : whole;
     DeviceCtx::StreamWorkspace* spare = nullptr;   // smallest one with memory that is large enough
     DeviceCtx::StreamWorkspace* empty = nullptr;
     for (auto& w : ctx->stream_workspaces) {
@@ -190,32 +188,83 @@ bool stream_workspace(DeviceCtx* ctx, cudaStream_t s, size_t bytes, float** ws, 
     return true;
 }
 
-CallMemory::CallMemory(DeviceCtx* ctx, cudaStream_t s, size_t bytes) : stream_(s) {
-    if (s == cudaStreamPerThread) return;   // as of stream_workspace
-    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(s, &status) != cudaSuccess) { (void)cudaGetLastError(); return; }
-    if (status != cudaStreamCaptureStatusNone) {
-        float* ws = nullptr;
-        uint32_t* counters;
-        if (stream_workspace(ctx, s, bytes, &ws, &counters)) ptr_ = ws;
-        return;
-    }
-    if (!ctx->call_pool) return;
-    RelaxedCapture relaxed;
-    cudaError_t e = cudaMallocFromPoolAsync(&ptr_, bytes, ctx->call_pool, s);
+namespace {
+// In the order of `s`; nullptr where there is none to be had.
+void* from_call_pool(DeviceCtx* ctx, size_t bytes, cudaStream_t s) {
+    void* ptr = nullptr;
+    cudaError_t e = cudaMallocFromPoolAsync(&ptr, bytes, ctx->call_pool, s);
     if (e == cudaErrorMemoryAllocation) {   // what the pool keeps in other sizes may be what is missing
         (void)cudaGetLastError();
         (void)cudaMemPoolTrimTo(ctx->call_pool, 0);
-        e = cudaMallocFromPoolAsync(&ptr_, bytes, ctx->call_pool, s);
+        e = cudaMallocFromPoolAsync(&ptr, bytes, ctx->call_pool, s);
     }
-    if (e != cudaSuccess) { (void)cuda_fail(e); ptr_ = nullptr; return; }
-    pooled_ = true;
+    if (e == cudaSuccess) return ptr;
+    (void)cuda_fail(e);
+    return nullptr;
+}
+void to_call_pool(void* ptr, cudaStream_t s) {
+    const cudaError_t e = cudaFreeAsync(ptr, s);
+    if (e != cudaSuccess) (void)cuda_fail(e);
+}
+
+// A capture's calls on one stream follow one another in the graph, so they share: the memory of the largest so far.  (Allocated as a node of the graph it would
+// forbid a second executable.)  It goes back when the graph and its executables are gone, at the next look at the list.
+void* graph_memory(DeviceCtx* ctx, cudaStream_t s, size_t bytes, unsigned long long capture, cudaGraph_t graph) {
+    for (auto* m = ctx->graph_memory; m; m = m->next)
+        if (m->stream == s && m->capture == capture && m->bytes >= bytes) return m->ptr;
+    auto* m = new (std::nothrow) DeviceCtx::GraphMemory;
+    auto* hold = new (std::nothrow) DeviceCtx::GraphHold;
+    void* ptr = m && hold ? from_call_pool(ctx, bytes, ctx->clear_stream) : nullptr;
+    cudaError_t e = ptr ? cudaStreamSynchronize(ctx->clear_stream) : cudaErrorMemoryAllocation;
+    cudaUserObject_t object = nullptr;
+    if (e == cudaSuccess) e = cudaUserObjectCreate(&object, hold, graph_gone, 1, cudaUserObjectNoDestructorSync);
+    if (e == cudaSuccess) {
+        *m = {ptr, bytes, s, capture, hold, ctx->graph_memory};
+        ctx->graph_memory = m;
+        e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+        if (e == cudaSuccess) return ptr;
+        m->capture = 0;   // nobody's any more
+        (void)cudaUserObjectRelease(object, 1);   // its half of `hold` goes with it, the list's at the next look at it
+    } else {
+        if (ptr) to_call_pool(ptr, ctx->clear_stream);
+        delete m;
+        delete hold;
+    }
+    (void)cuda_fail(e);
+    return nullptr;
+}
+void reclaim_graph_memory(DeviceCtx* ctx) {
+    for (auto** at = &ctx->graph_memory; *at;) {
+        auto* m = *at;
+        if (!m->hold->gone.load(std::memory_order_acquire)) { at = &m->next; continue; }
+        to_call_pool(m->ptr, ctx->clear_stream);
+        m->hold->release();
+        *at = m->next;
+        delete m;
+    }
+}
+}  // namespace
+
+CallMemory::CallMemory(DeviceCtx* ctx, cudaStream_t s, size_t bytes) : stream_(s) {
+    if (s == cudaStreamPerThread || !ctx->call_pool) return;   // cudaStreamPerThread: as of stream_workspace
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    cudaGraph_t graph = nullptr;
+    if (cudaStreamGetCaptureInfo(s, &status, &id, &graph) != cudaSuccess) { (void)cudaGetLastError(); return; }
+    if (status == cudaStreamCaptureStatusInvalidated) return;
+    RelaxedCapture relaxed;
+    {
+        std::lock_guard<std::mutex> lock(g_mutex);
+        if (ctx->graph_memory) reclaim_graph_memory(ctx);
+        if (status == cudaStreamCaptureStatusActive) { ptr_ = graph_memory(ctx, s, bytes, id, graph); return; }
+    }
+    ptr_ = from_call_pool(ctx, bytes, s);
+    pooled_ = ptr_ != nullptr;
 }
 CallMemory::~CallMemory() {
     if (!pooled_) return;
     RelaxedCapture relaxed;
-    const cudaError_t e = cudaFreeAsync(ptr_, stream_);
-    if (e != cudaSuccess) (void)cuda_fail(e);
+    to_call_pool(ptr_, stream_);
 }
 
 const DeviceCtx::Workspace* workspace_for(DeviceCtx* ctx, cudaStream_t s, int* rc) {
@@ -358,6 +407,12 @@ int afb_finalize(void) {
     cudaFree(c.status); cudaFree(c.ar_words); cudaFree(c.phase_ts);
     for (auto& w : c.workspaces) { if (w.ws) cudaFree(w.ws); if (w.counters) cudaFree(w.counters); }
     for (auto& w : c.stream_workspaces) { if (w.counters) cudaFree(w.counters); if (w.hold) w.hold->release(); }
+    while (auto* m = c.graph_memory) {
+        c.graph_memory = m->next;
+        to_call_pool(m->ptr, c.clear_stream);
+        m->hold->release();
+        delete m;
+    }
     if (c.clear_stream) cudaStreamDestroy(c.clear_stream);
     if (c.call_pool) cudaMemPoolDestroy(c.call_pool);
     for (int j = 0; j < 2; ++j) {

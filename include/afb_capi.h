@@ -136,7 +136,7 @@ int afb_device_sync(void);
  * so it must not run next to launches on that stream or to other graphs captured on it.
  * The streaming form of both variants (stream.cu: mostly 4 to 128 rows of large matrices) and the pair form (pair.cu: mostly from 65 rows,
  * and the fused launches) have workspaces of their own: one per stream for both (39 MB; afb_init allocates the first) and one per captured
- * graph (4 to 39 MB, by need; products grouped by expert up to 1 GB): such graphs may run next to each other and to their capture stream.  The first 32 captured graphs
+ * graph (4 to 39 MB, by need): such graphs may run next to each other and to their capture stream.  The first 32 captured graphs
  * keep theirs until afb_finalize; a further graph's goes back to the library when the graph and its executables are destroyed,
  * which costs its replays 2.5 us each.  (Two executables of ONE graph share its workspace; an executable
  * updated from another graph uses that graph's, which must then outlive it.)  They are allocated when first needed, also
@@ -257,9 +257,9 @@ int afb_moe_route_launch(const afb_moe_route_args* args, void* stream);
  * multiply the weights, in fp16: the product is exact for int4 without zero-points and bf16 scales, else off by 2^-11 of itself at most (2^-10 for fp32
  * scales); rows of A and the scales of a channel are given a power of two for that, and of the row's values what is below 2^-28 of the largest (of the
  * scales 2^-20) keeps fewer bits.  This form converts the rows of A first, into a_rows * k * 2 bytes and a little that the call takes and gives back in
- * the order of the stream (cudaMallocFromPoolAsync; the library's pool keeps up to 1 GB of what was used); inside a capture into a workspace of
- * the graph, as the streaming form has one.  Where there is no such memory to be had, and on cudaStreamPerThread, the other form runs
- * (afb_expert_many_launch_count tells).
+ * the order of the stream (cudaMallocFromPoolAsync; the library's pool keeps up to 1 GB of what was used).  Inside a capture the memory is the graph's, one for
+ * all its calls on a stream (two executables of one graph share it), and goes back when the graph and its executables are destroyed, which
+ * costs each replay 2.5 us.  Where there is no such memory to be had, and on cudaStreamPerThread, the other form runs (afb_expert_many_launch_count tells).
  * The offsets are read on the GPU.  They must not fall; values outside 0 .. m are taken as the nearer end.  A row(r) outside
  * 0 .. a_rows - 1 reads as a row of zeros. */
 typedef struct afb_expert_gemm_args {

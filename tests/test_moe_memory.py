@@ -1,5 +1,6 @@
 """Memory that a product grouped by expert hands its rows through from its first kernel to its second (group scales, form for many rows): whose it is, when it
 goes back, what is left for others."""
+import gc
 import threading
 
 import pytest
@@ -10,7 +11,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 from test_moe import Experts, activations, check, offsets_of  # noqa: E402
-from test_workspaces import STREAMING, Gemm  # noqa: E402
+from test_workspaces import STREAMING, Gemm, _new_streams  # noqa: E402
 
 MANY = dict(variant=pkg.VARIANT_PREFILL)
 
@@ -54,3 +55,111 @@ def test_two_threads_on_one_stream(afb, on):
     for outs, want, _ in jobs:
         assert all(torch.equal(out, want) for out in outs)
     assert afb.read_status()[0] == 0
+
+
+class Prompt:
+    """A product whose converted rows take rows * 8 KB."""
+
+    def __init__(self, afb, rows, seed=5):
+        self.afb, self.x = afb, Experts(4, 64, 4096, 4, 128, seed=seed)
+        self.a, self.offsets = torch.randn((rows, 4096), device="cuda").bfloat16(), offsets_of([rows // 4] * 3 + [rows - rows // 4 * 3])
+        self.want = self.run()
+        some = torch.cat([torch.arange(300), torch.arange(rows - 300, rows)]).cuda() if rows > 600 else torch.arange(rows).cuda()
+        ends = torch.tensor([0] + [int((some < o).sum()) for o in self.offsets[1:]], dtype=torch.int32, device="cuda")
+        check(self.want[some], *self.x.plain(self.a[some], ends, **MANY))
+
+    def run(self, out=None, stream=None):
+        before = self.afb.expert_many_launch_count()
+        out = self.x.run(self.afb, self.a, self.offsets, out=out, stream=torch.cuda.current_stream().cuda_stream if stream is None else stream, **MANY)
+        assert self.afb.expert_many_launch_count() == before + 1, "the form for few rows took the call"
+        return out
+
+    def captured(self, stream=None):
+        out, graph = torch.zeros_like(self.want), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            self.run(out)
+        return graph, out
+
+
+def held_since(start):
+    gc.collect()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    return start - torch.cuda.mem_get_info()[0]
+
+
+def streaming_on_new_streams(afb, dense, count):
+    before = afb.stream_launch_count()
+    for s in _new_streams(afb, count):
+        dense.launch(s)
+        dense.check("dense product on a new stream")
+    return afb.stream_launch_count() - before == count
+
+
+def test_growing_prompts_on_many_streams_leave_the_dense_products_theirs(afb):
+    """Rows of 75 MB to 0.6 GB, one call on each of twelve streams: every call in the form for many rows; nothing of it stays beyond the 1 GB that the pool keeps, and
+    the streaming form still finds its workspaces."""
+    dense = Gemm(afb, *STREAMING, seed=22)
+    start = held_since(0) * -1
+    for rows in (9216, 18500, 37000, 74000):
+        p = Prompt(afb, rows)
+        for s in _new_streams(afb, 3):
+            out = torch.zeros_like(p.want)
+            torch.cuda.synchronize()
+            p.run(out, s)
+            torch.cuda.synchronize()
+            assert torch.equal(out, p.want)
+        del p, out
+    assert held_since(start) <= (1024 + 64) << 20
+    assert streaming_on_new_streams(afb, dense, 8)
+
+
+def test_a_call_above_a_gigabyte(afb):
+    rows = 131072 + 900
+    Prompt(afb, rows)   # asserts that the form for many rows took it, and compares its first and last rows
+
+
+def test_captured_graphs_give_their_memory_back(afb):
+    """24 graphs of 151 MB each, alive at the same time: the form for many rows in all of them, workspaces left for the dense products.  Destroyed, they leave no more than
+    the pool keeps; graphs captured after them, in the memory that they had, do not disturb one that lives."""
+    dense, p, first = Gemm(afb, *STREAMING, seed=23), Prompt(afb, 18500), Prompt(afb, 700, seed=8)
+    start = held_since(0) * -1
+    stays = first.captured()
+    graphs = [p.captured() for _ in range(24)]
+    assert held_since(start) > 24 * 144 - 1024 << 20   # 18500 rows of 8 KB are 144.5 MiB; up to 1 GiB of them were the pool's before
+    assert streaming_on_new_streams(afb, dense, 8)
+    for graph, out in graphs[::5] + [stays]:
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, p.want) for _, out in graphs[::5]) and torch.equal(stays[1], first.want)
+    del graphs, graph, out
+    gc.collect()
+    torch.cuda.synchronize()
+    p.run()   # the library looks for memory of graphs that are gone
+    assert held_since(start) <= (1024 + 128) << 20
+    graph, out = p.captured()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            graph.replay()
+        stays[1].zero_()
+        stays[0].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, p.want) and torch.equal(stays[1], first.want)
+        out.zero_()
+    assert afb.read_status()[0] == 0
+
+
+def test_a_layer_captured_with_sizes_that_grow_and_shrink(afb):
+    """The calls of one capture share the memory of the largest so far."""
+    prompts = [Prompt(afb, rows, seed=rows) for rows in (300, 5000, 40, 2000, 9000)]
+    outs, graph = [torch.zeros_like(p.want) for p in prompts], torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for p, out in zip(prompts, outs):
+            p.run(out)
+    for _ in range(2):
+        for out in outs:
+            out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, p.want) for p, out in zip(prompts, outs))
