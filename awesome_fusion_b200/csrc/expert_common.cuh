@@ -112,14 +112,16 @@ __device__ __forceinline__ uint32_t source_row(const ExpertParams& p, uint32_t r
     return pair < 0 ? 0xffffffffu : (uint32_t)pair / p.top_k;
 }
 
-// v / (1 + exp(-v)) for a result that is rounded to bf16: the product -v log2(e) is rounded once, so the exponential is off by |v| 2^-24 and a little (2^-17 at
-// |v| = 87, where it leaves fp32), a 500th of the rounding to come.  (sigmoid() of pair.cu has three times the instructions: the drain of an accumulator of 256
-// gated columns waits for them.)  Below -128 infinity gives -0, at -infinity NaN, as the quotient would.
+// v / (1 + exp(-v)) for a result that is rounded to bf16, as v * (2^-16 / (2^-16 + 2^(-v log2(e) - 16))): the factor keeps the sum below 2^126, from where on rcp
+// returns 0, down to v = -98.4; the result is below half of the smallest bf16 there (without the factor it is lost from -87.3 on, -1e-36).  The argument is rounded
+// once, so the exponential is off by 2^-17 at most (2^-20 for |v| < 11), a 200th of the rounding to come; below v = -87.3, where the quotient leaves the normal range,
+// it loses bits towards 2^-149, as the result does towards 2^-133.  Infinite exponentials give -0, v = -infinity NaN, as the quotient would.
+// (sigmoid() of pair.cu has more than twice the instructions: the drain of an accumulator of 256 gated columns waits for them.)
 __device__ __forceinline__ float silu(float v) {
     float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.44269504f));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-    return v * r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(v, -1.44269504f, -16.f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(0x1p-16f + e));
+    return v * (r * 0x1p-16f);
 }
 
 // `bits`, `group`: of the weights.  For group scales the form for many rows needs a workspace; *done = false: there is none to be had, and nothing has

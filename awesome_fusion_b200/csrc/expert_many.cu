@@ -17,7 +17,7 @@
 // room for them: a weight of 4 bits times a scale of 8 has up to 12 significant ones, and a rounding to 8 costs as much accuracy as the rounding of the
 // result.  So these products are made in fp16, with 11: int4 without zero-points exactly (|q| <= 8 has three significant bits), with them and int8 off by
 // 2^-11 at most.  What fp16 lacks is range, so a kernel ahead of this one gives every row of A a power of two that brings its largest value below 2^15 (what is
-// below 2^-28 of it loses bits: 2^-40 of the largest at most), and finds one for every channel's scales (below 2^-20 of the largest they lose bits); the
+// below 2^-28 of it loses bits: 2^-39 of the largest at most), and finds one for every channel's scales (below 2^-20 of the largest they lose bits); the
 // epilogue takes both out again.  (Tried before: sums of each group in accumulators of their own, scaled and added in fp32 registers, which is exact, too:
 // 1650 cycles per step of 128 rows, the chain from accumulator to registers and back; 2048 tokens, 64 experts of 2048 x 4096 int4: 516 us.)
 //
