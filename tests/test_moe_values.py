@@ -46,3 +46,29 @@ def test_silu(afb, variant, group, gated):
     ok = off <= 2.0 ** -8 * (want.abs() + own) + 2.0 ** -134 + own + lost
     assert ok.all(), [(x[i].item(), got[i].item(), want[i].item()) for i in (~ok).nonzero()[:5, 0].tolist()]
     assert afb.read_status()[0] == 0
+
+
+@pytest.mark.parametrize("variant", FORMS)
+@pytest.mark.parametrize("fmt", [dict(bits=4, group=128), dict(bits=8, group=64, scale_f32=True), dict(bits=4, group=64, zero=True, packed=True)],
+                         ids=lambda f: "-".join(f"{k}{v}" for k, v in f.items()))
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("scales, rows", [(100, -70), (124, -104), (-90, 100), (-60, 20)])
+def test_ends_of_the_range_of_group_scales(afb, variant, fmt, gated, scales, rows):
+    """Scales of up to 2^118 on rows of 2^-104: the results are ordinary numbers, and no intermediate value may leave fp32 (sums of 2^29 in the kernel's units times
+    2^104 does).  Bounds: as of the ordinary range, and what A loses in fp16, 2^-39 of the row's largest value for each weight."""
+    from test_moe import Experts, activations, offsets_of
+    from test_moe_finite import check
+    x = Experts(2, 72, 512, seed=41, **fmt)
+    a, offsets = (activations(70, 512).float() * 2.0 ** rows).bfloat16(), offsets_of([3, 67])
+    x.scale = (x.scale.float() * 2.0 ** scales).to(x.scale.dtype)
+    x.w = x.w * 2.0 ** scales
+    want, off = x.plain(a, offsets, gated=gated, variant=variant)
+    if variant == pkg.VARIANT_PREFILL:
+        lost = torch.cat([2.0 ** -39 * a[lo:hi].double().abs().amax(1, keepdim=True) * x.w[e].abs().sum(1) for e, (lo, hi) in enumerate([(0, 3), (3, 70)])])
+        if gated:   # silu(gate) * up: the slope of silu is below 1.1
+            v = torch.cat([a[lo:hi].double() @ x.w[e].T for e, (lo, hi) in enumerate([(0, 3), (3, 70)])])
+            g, u = v[:, 0::2], v[:, 1::2]
+            lost = 1.1 * lost[:, 0::2] * (u.abs() + lost[:, 1::2]) + (g.abs() + 1.1 * lost[:, 0::2]) * lost[:, 1::2]
+        off = off + 1.01 * lost
+    check(x.run(afb, a, offsets, gated=gated, variant=variant), want, off)
+    assert afb.read_status()[0] == 0
