@@ -49,10 +49,6 @@ __device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint3
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-// `bytes` (0 or 16) from src, zeros behind them.
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 // The unpack's addend for a zero-point byte: -(the byte as an unsigned weight) * 2^-6, by the unpack's own multiply-add.
 template <int BITS> __device__ __forceinline__ uint32_t zero_addend(uint32_t zbyte, uint32_t flip) {
     const uint32_t u = (zbyte ^ flip) & (BITS == 8 ? 0xffu : 0xfu);
@@ -145,7 +141,7 @@ expert_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const FewParams p)
                 r.step(1, kStages);
             }
         }
-        cp_async_wait<0>();   // never leave with a copy still writing this CTA's shared memory
+        cp_async_wait_all();   // never leave with a copy still writing this CTA's shared memory
         for (uint32_t s = 0; s < kStages; ++s)
             if (issued & (1u << s)) ptx::mbar_wait(full(s), (parity >> s) & 1u);
     } else {

@@ -49,7 +49,7 @@ __host__ __device__ constexpr uint32_t regs_all(bool heavy) {
     return 128 * r.ctrl + 32 * kEpiWarps * r.epi + 128 * kConvGroups * r.conv + 32 * kLoadWarps * r.load;
 }
 static_assert(regs_all(false) <= 64u * kManyThreads && regs_all(true) <= 64u * kManyThreads, "shares of the registers");
-constexpr int kMaxRaw = 12, kMaxSlots = 8, kMaxAcc = 2;
+constexpr int kMaxRaw = 12, kMaxSlots = 8, kMaxAcc = 2;   // kMaxAcc: one accumulator per issuer
 __host__ __device__ constexpr uint32_t slots(int ks, bool low) { return ks == 128 && !low ? 4 : 6; }   // steps under way, in 256 columns at most (low strips: 384)
 constexpr uint32_t kTmemCols = 512;
 constexpr int kBars = 2 * (kMaxRaw + kMaxSlots + kMaxAcc);
@@ -70,11 +70,6 @@ struct ManyParams {
     const float* channel_mult;
     int32_t* status;
 };
-
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
-}
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // Two fp16 values at a time.
 __device__ __forceinline__ uint32_t f16x2_mul(uint32_t a, uint32_t b) {
@@ -200,7 +195,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
     constexpr uint32_t kSlots = slots(KS, LOW);
     constexpr Shares kShares = shares(BITS == 4 && GROUPED);
     constexpr uint32_t kIssuers = LOW ? 2 : 1;
-    static_assert(!LOW || (kConvGroups % 2 == 0 && kSlots % 2 == 0), "a slot's steps are one issuer's");
+    static_assert(!LOW || (KS == 128 && kConvGroups % 2 == 0 && kSlots % 2 == 0), "a slot's steps are one issuer's");
     extern __shared__ uint8_t smem_raw_base[];
     const uint32_t smem_base = (ptx::smem_u32(smem_raw_base) + 1023u) & ~1023u;
     uint8_t* smem_gen = smem_raw_base + (smem_base - ptx::smem_u32(smem_raw_base));
@@ -287,13 +282,13 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
             const uint32_t who = (uint32_t)warp - 2;
             const uint64_t desc0 = ptx::umma_desc_kmajor_sw128(smem_base + off_act);
             r.i = who;
-            Ring rc{0, 0};   // the accumulator(s): a ring of one
+            uint32_t acc_phase = 0;
             uint32_t before = 0, g = who;   // steps of the tiles walked so far; this warp's next step, counted over all tiles
             bool ready = false;
             while (ok && next(x)) {
                 const uint32_t idesc = GROUPED ? ptx::umma_idesc_f16_f32(2 * kCh, x.height) : ptx::umma_idesc_bf16_f32(2 * kCh, x.height), slab_d = x.height * 64u >> 4;
                 const uint32_t td = tmem_base + who * acc_cols, acc_done = acc_full(who), first = g;
-                if (!warp_wait(acc_empty(who), rc.phase ^ 1u, abort_flag)) { give_up(63, x.expert, 0); break; }
+                if (!warp_wait(acc_empty(who), acc_phase ^ 1u, abort_flag)) { give_up(63, x.expert, 0); break; }
                 for (; g < before + ns; g += kIssuers) {
                     if (!__all_sync(0xffffffffu, ready) && !warp_wait(step_full(r.i), r.phase, abort_flag)) { give_up(64, x.expert, g); ok = false; break; }
                     ptx::fence_proxy_async_smem();
@@ -311,7 +306,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                     }
                 }
                 before += ns;
-                rc.step(1, 1);
+                acc_phase ^= 1u;
             }
         } else if (warp == 2) {
             // ======================= rank 1: reports its half of each step =======================
@@ -480,7 +475,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                     const bool there = src[i] < p.x.a_rows;
                     const uint16_t* row = there ? from + (size_t)src[i] * p.x.lda : p.x.a;
 #pragma unroll
-                    for (int h = 0; h < KS / kSlab; ++h) cp_async16_or_zero(to + h * slab_bytes + i * 2048u, row + (there ? h * kSlab : 0), there);
+                    for (int h = 0; h < KS / kSlab; ++h) cp_async16_or_zero(to + h * slab_bytes + i * 2048u, row + (there ? h * kSlab : 0), there ? 16u : 0u);
                 }
                 cp_async_arrive(step_full(r.i));
                 issued |= 1u << r.i; parity = (parity & ~(1u << r.i)) | (r.phase << r.i);
@@ -497,7 +492,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
         constexpr int kPacks = LOW ? 2 : 8;   // of 16 columns: this warp's half of a strip
         const bool odd = lane & 1, gated = p.x.gated != 0, act = p.x.silu != 0;
         const uint32_t stage = smem_base + kOffOut + (uint32_t)(warp - kFirstEpi) * 2 * kOutBytes;
-        Ring rc{0, 0};   // the accumulator(s): a ring of one
+        uint32_t acc_phase = 0;
         bool ok = true;
         auto drained = [&] {   // everything of the accumulator is in registers
             ptx::tc_fence_before_sync();
@@ -561,8 +556,8 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                 const uint32_t row = i * 32 + lane < valid ? p.x.row_pair ? source_row(p.x, x.row0 + first + i * 32 + lane) : x.row0 + first + i * 32 + lane : 0xffffffffu;
                 factor[i] = GROUPED && row < p.x.a_rows ? p.row_factor[row] * 512.f : 0.f;
             }
-            if (!warp_wait(acc_full(0), rc.phase, abort_flag)) { give_up(68, x.expert, 0); break; }
-            if (LOW && !warp_wait(acc_full(1), rc.phase, abort_flag)) { give_up(68, x.expert, 1); break; }
+            if (!warp_wait(acc_full(0), acc_phase, abort_flag)) { give_up(68, x.expert, 0); break; }
+            if (LOW && !warp_wait(acc_full(1), acc_phase, abort_flag)) { give_up(68, x.expert, 1); break; }
             ptx::tc_fence_after_sync();
 #pragma unroll
             for (int i = 0; i < kPacks; ++i) {
@@ -586,7 +581,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                 finish(o[i], v, 16 * i);
             }
             drained();
-            rc.step(1, 1);
+            acc_phase ^= 1u;
             // Blocks of 16 rows turn round in shared memory and leave in 16-byte pieces, 64 (gated 32) contiguous bytes a row; two blocks take turns.
             const uint32_t c0 = x.n0 + quarter * 32u;   // first channel of this warp
             if (c0 >= p.x.n) continue;
@@ -678,7 +673,9 @@ int launch_many(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uint3
 
 template <int BITS, bool GROUPED, int KS>
 int launch_cfg(const CUtensorMap& tw, const ManyParams& p, uint32_t grid, uint32_t smem, DeviceCtx* ctx, cudaStream_t s) {
-    return p.x.tile_rows <= 64 ? launch_many<BITS, GROUPED, KS, true>(tw, p, grid, smem, ctx, s) : launch_many<BITS, GROUPED, KS, false>(tw, p, grid, smem, ctx, s);
+    if constexpr (KS == 128)   // k an odd multiple of 64 leaves a raw block that is not whole: no low strips
+        if (p.x.tile_rows <= 64) return launch_many<BITS, GROUPED, KS, true>(tw, p, grid, smem, ctx, s);
+    return launch_many<BITS, GROUPED, KS, false>(tw, p, grid, smem, ctx, s);
 }
 
 }  // namespace
