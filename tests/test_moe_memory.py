@@ -163,3 +163,48 @@ def test_a_layer_captured_with_sizes_that_grow_and_shrink(afb):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(out, p.want) for p, out in zip(prompts, outs))
+
+
+def test_calls_next_to_a_capture_elsewhere(afb):
+    """While one thread captures in global mode, another one's calls take and give back memory on streams that are new to the library."""
+    p = Prompt(afb, 3000, seed=9)
+    streams, outs, failed, x, graph = _new_streams(afb, 4), [torch.zeros_like(p.want) for _ in range(4)], [], torch.zeros(8, device="cuda"), torch.cuda.CUDAGraph()
+
+    def calls():
+        try:
+            for s, out in zip(streams, outs):
+                p.run(out, s)
+        except Exception as e:   # noqa: BLE001
+            failed.append(e)
+
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        x += 1
+        t = threading.Thread(target=calls)
+        t.start()
+        t.join()
+        x += 1
+    torch.cuda.synchronize()
+    assert not failed and all(torch.equal(out, p.want) for out in outs)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert x.tolist() == [2.0] * 8
+
+
+def test_finalize_with_a_captured_graph_alive(afb):
+    """The graph's half of what it holds outlives the library's; after a new afb_init calls and captures work as before."""
+    p = Prompt(afb, 900, seed=10)
+    graph, out = p.captured()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, p.want)
+    afb.finalize()
+    del graph
+    gc.collect()
+    torch.cuda.synchronize()
+    afb.init(0)
+    assert torch.equal(p.run(), p.want)
+    graph, out = p.captured()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, p.want)
