@@ -517,9 +517,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
             // channel and exchange half of the 16 rows: the even lane finishes rows 0 to 7, the odd one 8 to 15.
             uint32_t o[kPacks][8];
             float factor[4] = {};   // group scales: what rows lane, lane + 32, ... have to be multiplied by
-            float scale, other_scale = 0.f;   // of this lane's channel; gated: of the other one of the pair
-            // Group scales: the powers of two of channel and row are multiplied first, where none of what a result in range needs is lost.
-            auto row_scaled = [&](float v, uint32_t row) { return GROUPED ? v * (scale * __shfl_sync(0xffffffffu, factor[row / 32], row)) : v; };
+            auto row_scaled = [&](float v, uint32_t row) { return GROUPED ? v * __shfl_sync(0xffffffffu, factor[row / 32], row) : v; };
             auto finish = [&](uint32_t (&to)[8], const float (&v)[16], int at) {   // at: the first of the 16 rows
                 if (gated) {
 #pragma unroll
@@ -530,8 +528,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                             const float lo = v[j + i], hi = v[j + i + 8], other = __shfl_xor_sync(0xffffffffu, odd ? lo : hi, 1);
                             // the two lanes of a pair have different rows: the factor is fetched from the lane that knows it
                             const float fr = GROUPED ? __shfl_sync(0xffffffffu, factor[at / 32], at % 32 + j + i + (odd ? 8 : 0)) : 1.f;
-                            const float gate = GROUPED ? (odd ? other : lo) * ((odd ? other_scale : scale) * fr) : odd ? other : lo;
-                            const float up = GROUPED ? (odd ? hi : other) * ((odd ? scale : other_scale) * fr) : odd ? hi : other;
+                            const float gate = (odd ? other : lo) * fr, up = (odd ? hi : other) * fr;
                             f[i] = (act ? silu(gate) : gate) * up;
                         }
                         to[j / 2] = pack2(f[0], f[1]);
@@ -547,14 +544,20 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
             const uint32_t column = tmem_base + ((quarter * 32u) << 16) + half * cols;
             // Per channel the sum of products times the scale; of group scales the powers of two that channel and row were given.
             const uint32_t first = half * cols, valid = x.rows > first ? min(cols, x.rows - first) : 0u;
-            scale = GROUPED ? 1.f / p.channel_mult[chan]
-                            : p.x.scale_dtype == AFB_SCALE_BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.x.scale)[chan] << 16)
-                                                                : reinterpret_cast<const float*>(p.x.scale)[chan];
-            if (GROUPED) other_scale = __shfl_xor_sync(0xffffffffu, scale, 1);
+            float scale = GROUPED ? 1.f / p.channel_mult[chan]
+                                  : p.x.scale_dtype == AFB_SCALE_BF16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p.x.scale)[chan] << 16)
+                                                                      : reinterpret_cast<const float*>(p.x.scale)[chan];
+            // A sum, up to 2^53, meets the channel's power first: none of the warp's may be above 2^60, what is above goes to the rows' side.
+            int above = 0;
+            if (GROUPED) {
+                above = max((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(scale)) >> 23) - 127 - 60, 0);
+                scale *= power_of_two(-above);
+            }
+            const float unit = power_of_two(9 + above);   // 512: the weights' 2^-9
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
                 const uint32_t row = i * 32 + lane < valid ? p.x.row_pair ? source_row(p.x, x.row0 + first + i * 32 + lane) : x.row0 + first + i * 32 + lane : 0xffffffffu;
-                factor[i] = GROUPED && row < p.x.a_rows ? p.row_factor[row] * 512.f : 0.f;
+                factor[i] = GROUPED && row < p.x.a_rows ? fminf(p.row_factor[row] * unit, 0x1p127f) : 0.f;
             }
             if (!warp_wait(acc_full(0), acc_phase, abort_flag)) { give_up(68, x.expert, 0); break; }
             if (LOW && !warp_wait(acc_full(1), acc_phase, abort_flag)) { give_up(68, x.expert, 1); break; }
@@ -577,7 +580,7 @@ expert_many_kernel(const __grid_constant__ CUtensorMap tmap_w, const ManyParams 
                 }
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
-                    v[j] = GROUPED ? __uint_as_float(a[j]) : unscaled(__uint_as_float(a[j]), scale);
+                    v[j] = GROUPED ? __uint_as_float(a[j]) * scale : unscaled(__uint_as_float(a[j]), scale);
                 finish(o[i], v, 16 * i);
             }
             drained();
