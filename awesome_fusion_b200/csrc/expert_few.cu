@@ -17,7 +17,7 @@
 //
 // What bounds it.  int8 per channel: HBM (32 rows on 8 experts of 22016 x 4096, gated: 114 to 140 us with the experts' shares of the rows, 5.2 to 6.3 TB/s).  int4 in groups:
 // instructions, 650 to 780 per warp and stage of 4 KB, four warps a scheduler at 0.55 of the issue slots (8 rows on 8 experts of 2048 x 4096: 14 us, 2.4 TB/s
-// from L2; 16 rows each on 64 experts: 137 us, where the form for many rows takes 114).
+// from L2; 16 rows each on 64 experts: 133 us, where the form for many rows takes 112).
 #include "dequant.cuh"
 #include "decode_common.cuh"
 #include "expert_common.cuh"
@@ -446,6 +446,8 @@ extern "C" int afb_expert_gemm_launch(const afb_expert_gemm_args* x, void* strea
     //   64 experts of 2048 x 4096 gated, int4 group-128: 8 rows 86 / 97, 12: 110 / 112, 16: 133 / 112, 24: 165 / 126;  int8: 4: 82 / 80, 8: 102 / 92
     //   8 of 11008 x 4096, int4 group-128: 12: 74 / 85, 16: 88 / 85, 24: 121 / 85;  int8: 4: 82 / 80, 12: 88 / 80
     //   16 of 4096 x 2816, int4 group-64: 8: 50 / 54, 12: 59 / 54, 24: 80 / 56;  128 of 1536 x 2048, int8 group-128: 4: 72 / 81, 8: 92 / 87
+    // One threshold per width: between 8 and 12 int4 in groups of 64, between 4 and 8 int8 in groups take the slower form by a tenth at most.  m is the host's bound of the
+    // pairs: those of padded tokens count.
     const bool many = a.variant == AFB_VARIANT_PREFILL || (a.variant == AFB_VARIANT_AUTO && (uint64_t)a.m > (a.b_bits == 8 ? 4ull : 12ull) * x->experts);
     if (many) {
         bool done = false;

@@ -109,7 +109,7 @@ class DecodeGraph:
 #     out = torch.ops.afb.moe_combine(y, weights, pair_row, residual)
 #
 # include/afb_capi.h says what each computes.  Weights are [experts, N, K * bits / 8], scales [experts, N] or [experts, N, K / group_size],
-# zero-points (optional) uint8 of the scales' shape.  No host synchronisation; zero tokens are taken.
+# zero-points (optional) uint8 of the scales' shape.  No host synchronisation; zero tokens are taken.  The form of a product is AFB_VARIANT_AUTO's choice.
 
 def _on(t, name, device, dtypes, dim=None):
     if t.device != device or t.dtype not in dtypes or (dim is not None and t.dim() != dim):

@@ -247,7 +247,8 @@ int afb_moe_route_launch(const afb_moe_route_args* args, void* stream);
  *              [experts, n, k / group_size]
  *     b_layout AFB_LAYOUT_COL or AFB_LAYOUT_COL_PACKED (afb_prepack / afb_prepack_gated of all experts at once: a matrix of experts * n rows)
  *     group_size 0, or a power of two of at least 64;  k a multiple of 64 (int8) or 128 (int4);  lda a multiple of 8, A 16-byte aligned, rows
- *              of B and ptr_b 16-byte aligned; any n and ldc.  Otherwise AFB_ERR_UNSUPPORTED.  k < 2^24, m, a_rows and experts * n < 2^31
+ *              of B and ptr_b 16-byte aligned; any n and ldc.  Otherwise AFB_ERR_UNSUPPORTED (both forms read 64 bytes of a row of B at a time, which lie in one
+ *              group, or int4 in two; the [K,N] layout goes through afb_prepack).  k < 2^24, m, a_rows and experts * n < 2^31.  C must not overlap an input
  *     variant  AFB_VARIANT_AUTO, AFB_VARIANT_DECODE (form for few rows per expert: weights streamed through registers) or
  *              AFB_VARIANT_PREFILL (form for many: tcgen05);  flags 0.
  *     C[r,:] = f(A[row(r),:] x dequant(B[e])^T)   for offsets[e] <= r < offsets[e + 1]
@@ -256,10 +257,11 @@ int afb_moe_route_launch(const afb_moe_route_args* args, void* stream);
  * in fp32 from the fp32 sums, rounded to bf16 once.  Group scales multiply the fp32 sum of each group in the form for few rows.  In the form for many they
  * multiply the weights, in fp16: the product is exact for int4 without zero-points and bf16 scales, else off by 2^-11 of itself at most (2^-10 for fp32
  * scales); rows of A and the scales of a channel are given a power of two for that, and of the row's values what is below 2^-28 of the largest (of the
- * scales 2^-20) keeps fewer bits.  This form converts the rows of A first, into a_rows * k * 2 bytes and a little that the call takes and gives back in
+ * scales 2^-20) keeps fewer bits.  (The dense product's prefill variant rounds them to bf16, 2^-9.)  AFB_VARIANT_DECODE has the fp32 sums whatever the number of
+ * rows.  The form for many rows converts the rows of A first, into a_rows * k * 2 bytes and a little that the call takes and gives back in
  * the order of the stream (cudaMallocFromPoolAsync; the library's pool keeps up to 1 GB of what was used).  Inside a capture the memory is the graph's, one for
- * all its calls on a stream (two executables of one graph share it), and goes back when the graph and its executables are destroyed, which
- * costs each replay 2.5 us.  Where there is no such memory to be had, and on cudaStreamPerThread, the other form runs (afb_expert_many_launch_count tells).
+ * all its calls on a stream (two executables of one graph share it; one that is updated from another graph uses that graph's, which must outlive it),
+ * and goes back when the graph and its executables are destroyed, which costs each replay 2.5 us.  Where there is no such memory to be had, and on cudaStreamPerThread, the other form runs (afb_expert_many_launch_count tells).
  * The offsets are read on the GPU.  They must not fall; values outside 0 .. m are taken as the nearer end.  A row(r) outside
  * 0 .. a_rows - 1 reads as a row of zeros. */
 typedef struct afb_expert_gemm_args {
