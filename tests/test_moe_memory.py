@@ -208,3 +208,71 @@ def test_finalize_with_a_captured_graph_alive(afb):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, p.want)
+
+
+def test_a_full_device_takes_the_form_without(afb):
+    """Where the rows' memory is not to be had, eager or inside a capture, the form for few rows answers, and nothing of the refusal stays behind."""
+    p = Prompt(afb, 74000, seed=12)   # 0.6 GB
+    few = p.x.run(afb, p.a, p.offsets, variant=pkg.VARIANT_DECODE)
+    out, captured, graph = torch.zeros_like(few), torch.zeros_like(few), torch.cuda.CUDAGraph()
+    some = torch.ones(1, device="cuda")
+    torch.cuda.synchronize()
+    afb.finalize()   # the pool keeps nothing
+    afb.init(0)
+    torch.cuda.empty_cache()
+    full = torch.empty(torch.cuda.mem_get_info()[0] - (400 << 20), dtype=torch.uint8, device="cuda")
+    before = afb.expert_many_launch_count()
+    p.x.run(afb, p.a, p.offsets, out=out, **MANY)
+    with torch.cuda.graph(graph):
+        p.x.run(afb, p.a, p.offsets, out=captured, stream=torch.cuda.current_stream().cuda_stream, **MANY)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert afb.expert_many_launch_count() == before
+    assert torch.equal(out, few) and torch.equal(captured, few)
+    some += 1   # no error was left for the next launch
+    torch.cuda.synchronize()
+    del full
+    torch.cuda.empty_cache()
+    assert torch.equal(p.run(), p.want)
+    assert afb.read_status()[0] == 0 and some.item() == 2
+
+
+def test_a_graph_destroyed_while_it_runs(afb):
+    """Its memory goes to nobody else before its last launch has ended: calls on other streams look for memory meanwhile."""
+    p, q = Prompt(afb, 18500, seed=13), Prompt(afb, 18500, seed=14)
+    side, running = torch.cuda.Stream(), 0
+    for _ in range(5):
+        outs, graph = [torch.zeros_like(p.want) for _ in range(40)], torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for out in outs:
+                p.run(out)
+        other, end = [torch.zeros_like(q.want) for _ in range(8)], torch.cuda.Event()
+        torch.cuda.synchronize()
+        graph.replay()
+        end.record()
+        del graph
+        for out in other:
+            q.run(out, side.cuda_stream)
+        running += not end.query()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, p.want) for out in outs) and all(torch.equal(out, q.want) for out in other)
+    assert running, "the graph had always ended before the other calls were launched"
+
+
+def test_two_branches_of_one_graph(afb):
+    """A capture that forks: products on both streams run at the same time in the graph, each stream's in memory of its own."""
+    p, q, graph, side = Prompt(afb, 6000, seed=15), Prompt(afb, 6000, seed=16), torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    outs, others = ([torch.zeros_like(x.want) for _ in range(10)] for x in (p, q))
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        for out, other in zip(outs, others):
+            p.run(out, main.cuda_stream)
+            q.run(other, side.cuda_stream)
+        main.wait_stream(side)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, p.want) for out in outs) and all(torch.equal(out, q.want) for out in others)
+        for out in outs + others:
+            out.zero_()
